@@ -215,6 +215,60 @@ kd_attn_status kd_attn_qkv_projection(kd_attn_ctx* ctx, const kd_tensor* x, cons
  * y : [C, L, N] f32, bf16 or f16, rows contiguous and 16-byte aligned */
 kd_attn_status kd_attn_linear(kd_attn_ctx* ctx, const kd_tensor* x, const kd_linear* w, kd_tensor* y, void* stream);
 
+/* ------------------------------------------------------------------ 8-bit linear path
+ * No reference counterpart: kandinsky.cpp quantizes weights only (q8_0 / q4_0, expanded for every product).
+ * Here both operands of a Linear are 8-bit floating point with a scale per 128 columns, so that the tensor
+ * cores run at twice the 16-bit rate and a weight is read at one byte per element.
+ *
+ * kd_fp8_rows: `rows` rows of K columns.  codes: one e4m3 byte per element, row r at codes + r * nb1 (nb1 a
+ * multiple of 16, at least K rounded up to 16; codes 16-byte aligned; the bytes past K are not read).
+ * scales: for each row and block b of 128 columns a byte s, the block's scale being 2^(s - 127); the byte of
+ * (r, b) is at ((r / 128) * T + b / 4) * 512 + (r % 32) * 16 + (r % 128 / 32) * 4 + b % 4 with
+ * T = ceil(ceil(K / 128) / 4) (kd_attn_fp8_scale_bytes in all, 16-byte aligned): the order in which the
+ * tensor core takes them.  An element is worth code * 2^(s - 127).
+ *
+ * The writers choose the smallest scale >= 2^-126 with max|v| <= 448 * scale over the block and round codes to
+ * nearest even.  A NaN or an infinity becomes the NaN code and does not count for the scale.  Rows and columns
+ * outside the given sizes are left as they were, but for the up to 15 code bytes from K to the next multiple of 16.
+ * K is at most 2^20 and rows at most 2^24. */
+typedef struct {
+    void* codes;    /* device */
+    void* scales;   /* device */
+    int64_t ne[2];  /* {K, rows} */
+    size_t nb1;     /* bytes between rows of codes */
+} kd_fp8_rows;
+
+/* Bytes of the scales of K x rows. */
+kd_attn_status kd_attn_fp8_scale_bytes(int64_t K, int64_t rows, size_t* bytes);
+
+/* out (L * N rows, token l of sequence n = row n * L + l) = x in 8 bits.  x : [K, L, N] f32, f16 or bf16, any
+ * strides with dim 0 contiguous. */
+kd_attn_status kd_attn_quantize_fp8(kd_attn_ctx* ctx, const kd_tensor* x, kd_fp8_rows* out, void* stream);
+
+/* out (C rows of K) = the weight of a Linear in 8 bits, laid out once for kd_attn_linear_fp8.  Types as for
+ * kd_attn_linear; K a multiple of 32 for q8_0 / q4_0.  The bias is not read. */
+kd_attn_status kd_attn_quantize_weight_fp8(kd_attn_ctx* ctx, const kd_linear* w, kd_fp8_rows* out, void* stream);
+
+/* y : [K, L, N] f32, f16 or bf16 = the values of x (L * N rows), rounded once (bf16 holds all of them exactly
+ * while 2^(s - 127) stays above 2^-117). */
+kd_attn_status kd_attn_dequantize_fp8(kd_attn_ctx* ctx, const kd_fp8_rows* x, kd_tensor* y, void* stream);
+
+/* Root-mean-square norm of a residual stream into 8-bit rows: s = x + residual, out = s / sqrt(mean(s^2) + eps)
+ * * gain (RMSNorm, module.hpp:163-180, over whole rows).
+ * x : [K, L, N] f32, f16 or bf16, any strides with dim 0 contiguous, K at most 32768
+ * residual : as x (same type and sizes) or NULL
+ * gain : device f32 [K], or NULL for unit gain;  eps >= 0
+ * h : as x, or NULL: receives s, rounded to its type; the norm is taken of the rounded s whether or not h is
+ *     given.  h may be x or residual itself. */
+kd_attn_status kd_attn_rms_norm_fp8(kd_attn_ctx* ctx, const kd_tensor* x, const kd_tensor* residual,
+                                    const float* gain, float eps, kd_tensor* h, kd_fp8_rows* out, void* stream);
+
+/* ops::linear (ops.hpp:27-42) on 8-bit operands: y = x W^T + b, summed in f32 and rounded once.
+ * x : L * N rows of K;  w : C rows of K, any C;  bias : device f32 [C] or NULL
+ * y : [C, L, N] f32, bf16 or f16, any strides with dim 0 contiguous, not overlapping the operands. */
+kd_attn_status kd_attn_linear_fp8(kd_attn_ctx* ctx, const kd_fp8_rows* x, const kd_fp8_rows* w, const float* bias,
+                                  kd_tensor* y, void* stream);
+
 /* Replaces DiTSelfAttention::forward (crossdit.hpp:117-154) from the hidden states to the block output:
  * kd_attn_qkv_projection (bf16 operands), the flash kernel (scale 1/sqrt(d), no mask) and the
  * out-projection, with the intermediate tensors in the context's scratch.

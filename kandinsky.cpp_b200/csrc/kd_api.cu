@@ -1267,6 +1267,221 @@ kd_attn_status linear_core(kd_attn_ctx* ctx, const kd_tensor* x, const kd_linear
     return gemm_run(ctx, in, ws, p, nullptr, y->type, work, st);
 }
 
+// ------------------------------------------------------------------ 8-bit linear path
+constexpr int64_t kFp8MaxCols = 1 << 20, kFp8MaxRows = 1 << 24;
+
+int64_t fp8_ktiles(int64_t K) { return ((K + 127) / 128 + 3) / 4; }
+
+kd_attn_status check_fp8_rows(kd_attn_ctx* ctx, const kd_fp8_rows* r, const char* name, Fp8Rows* out) {
+    if (!r) return fail(ctx, KD_ATTN_ERR_INVALID_ARGUMENT, "%s is NULL", name);
+    if (r->ne[0] <= 0 || r->ne[1] < 0)
+        return fail(ctx, KD_ATTN_ERR_INVALID_ARGUMENT, "%s: %lld columns, %lld rows", name, (long long)r->ne[0],
+                    (long long)r->ne[1]);
+    if (r->ne[0] > kFp8MaxCols || r->ne[1] > kFp8MaxRows)
+        return fail(ctx, KD_ATTN_ERR_UNSUPPORTED, "%s: more than 2^20 columns or 2^24 rows", name);
+    const int64_t Kp = (r->ne[0] + 15) / 16 * 16;
+    const bool one = r->ne[1] <= 1;  // the stride of a single row is not used
+    if (!one && ((int64_t)r->nb1 < Kp || r->nb1 % 16 || r->nb1 > (size_t)1 << 32))
+        return fail(ctx, KD_ATTN_ERR_INVALID_ARGUMENT,
+                    "%s: rows are %zu bytes apart: a multiple of 16 from %lld is needed", name, r->nb1, (long long)Kp);
+    if (r->ne[1] && (!r->codes || !r->scales))
+        return fail(ctx, KD_ATTN_ERR_INVALID_ARGUMENT, "%s: codes or scales are NULL", name);
+    if (!aligned16(r->codes) || !aligned16(r->scales))
+        return fail(ctx, KD_ATTN_ERR_INVALID_ARGUMENT, "%s: codes and scales must be 16-byte aligned", name);
+    out->codes = static_cast<uint8_t*>(r->codes);
+    out->row_bytes = one ? Kp : (long long)r->nb1;
+    out->scales = static_cast<uint8_t*>(r->scales);
+    out->K = (int)r->ne[0];
+    out->Kp = (int)Kp;
+    out->ktiles = (int)fp8_ktiles(r->ne[0]);
+    out->rows = r->ne[1];
+    return KD_ATTN_OK;
+}
+
+// A [K, L, N] tensor of the 8-bit path: any strides that are whole elements; `written` rows may not overlap.
+struct TokenRows {
+    long long nb1 = 0, nb2 = 0, L = 1;
+    bool vec = false;  // rows start on 16-byte boundaries
+};
+kd_attn_status check_token_rows(kd_attn_ctx* ctx, const kd_tensor* t, const char* name, int64_t K, int64_t rows,
+                                bool written, TokenRows* out) {
+    kd_attn_status rc;
+    if ((rc = check_tensor(ctx, t, name))) return rc;
+    if (t->ne[3] != 1 || t->ne[0] != K || t->ne[1] * t->ne[2] != rows)
+        return fail(ctx, KD_ATTN_ERR_INVALID_ARGUMENT, "%s must be [%lld, L, N] with L * N = %lld rows", name,
+                    (long long)K, (long long)rows);
+    uint64_t nb[4];
+    packed_strides(t, nb);
+    const size_t es = elt_size(t->type);
+    if (reinterpret_cast<uintptr_t>(t->data) % es || nb[1] % es || nb[2] % es)
+        return fail(ctx, KD_ATTN_ERR_UNSUPPORTED, "%s: address or strides are not whole elements", name);
+    if (written && ((t->ne[1] > 1 && nb[1] < es * (uint64_t)K) || (t->ne[2] > 1 && nb[2] < es * (uint64_t)K)))
+        return fail(ctx, KD_ATTN_ERR_INVALID_ARGUMENT, "%s: its rows overlap", name);
+    out->nb1 = (long long)nb[1];
+    out->nb2 = (long long)nb[2];
+    out->L = t->ne[1] > 0 ? t->ne[1] : 1;
+    if (nb[2] == nb[1] * (uint64_t)t->ne[1] || t->ne[2] == 1) out->L = rows > 0 ? rows : 1;  // evenly spaced rows
+    out->vec = aligned16(t->data) && nb[1] % 16 == 0 && nb[2] % 16 == 0;
+    return KD_ATTN_OK;
+}
+
+kd_attn_status quantize_fp8_core(kd_attn_ctx* ctx, const kd_tensor* x, kd_fp8_rows* out, cudaStream_t st) {
+    kd_attn_status rc;
+    Quant8Params p{};
+    TokenRows tx;
+    if ((rc = check_fp8_rows(ctx, out, "out", &p.out)) ||
+        (rc = check_token_rows(ctx, x, "x", p.out.K, p.out.rows, false, &tx)))
+        return rc;
+    p.x = x->data;
+    p.x_nb1 = tx.nb1;
+    p.x_nb2 = tx.nb2;
+    p.x_vec = tx.vec;
+    p.L = tx.L;
+    KD_CUDA(ctx, launch_quant8(x->type, p, ctx->num_sms, st));
+    return KD_ATTN_OK;
+}
+
+kd_attn_status quantize_weight_fp8_core(kd_attn_ctx* ctx, const kd_linear* w, kd_fp8_rows* out, cudaStream_t st) {
+    kd_attn_status rc;
+    Fp8Rows o{};
+    if ((rc = check_fp8_rows(ctx, out, "out", &o))) return rc;
+    if (!w) return fail(ctx, KD_ATTN_ERR_INVALID_ARGUMENT, "w is NULL");
+    if (w->ne[0] != o.K || w->ne[1] != o.rows)
+        return fail(ctx, KD_ATTN_ERR_INVALID_ARGUMENT, "w is %lld x %lld and out is %d x %lld", (long long)w->ne[0],
+                    (long long)w->ne[1], o.K, o.rows);
+    const int64_t rb = weight_row_bytes(w->type, o.K);
+    if (rb < 0) return fail(ctx, KD_ATTN_ERR_UNSUPPORTED, "weight type %d is not f32/f16/bf16/q4_0/q8_0", w->type);
+    if (w->type != KD_ATTN_TYPE_Q8_0 && w->type != KD_ATTN_TYPE_Q4_0) {
+        kd_tensor x{};
+        x.data = const_cast<void*>(w->data);
+        x.type = w->type;
+        x.ne[0] = o.K;
+        x.ne[1] = o.rows;
+        x.ne[2] = x.ne[3] = 1;
+        x.nb[0] = elt_size(w->type);
+        x.nb[1] = w->nb1;
+        x.nb[2] = x.nb[3] = w->nb1 * (size_t)o.rows;
+        if ((int64_t)w->nb1 < rb) return fail(ctx, KD_ATTN_ERR_INVALID_ARGUMENT, "weight nb1 smaller than a row");
+        return quantize_fp8_core(ctx, &x, out, st);
+    }
+    if (o.K % 32) return fail(ctx, KD_ATTN_ERR_UNSUPPORTED, "in_features %d is not a multiple of 32", o.K);
+    if ((int64_t)w->nb1 < rb) return fail(ctx, KD_ATTN_ERR_INVALID_ARGUMENT, "weight nb1 smaller than a row");
+    if (o.rows && !w->data) return fail(ctx, KD_ATTN_ERR_INVALID_ARGUMENT, "weight data is NULL");
+    if (reinterpret_cast<uintptr_t>(w->data) % 2 || w->nb1 % 2)
+        return fail(ctx, KD_ATTN_ERR_UNSUPPORTED, "weight blocks must be 2-byte aligned");
+    KD_CUDA(ctx, launch_quant8_ggml(w->data, w->type == KD_ATTN_TYPE_Q4_0, (long long)w->nb1, o, ctx->num_sms, st));
+    return KD_ATTN_OK;
+}
+
+kd_attn_status dequantize_fp8_core(kd_attn_ctx* ctx, const kd_fp8_rows* x, kd_tensor* y, cudaStream_t st) {
+    kd_attn_status rc;
+    Dequant8Params p{};
+    TokenRows ty;
+    if ((rc = check_fp8_rows(ctx, x, "x", &p.in)) ||
+        (rc = check_token_rows(ctx, y, "y", p.in.K, p.in.rows, true, &ty)))
+        return rc;
+    p.y = y->data;
+    p.y_nb1 = ty.nb1;
+    p.y_nb2 = ty.nb2;
+    p.y_vec = ty.vec;
+    p.L = ty.L;
+    KD_CUDA(ctx, launch_dequant8(y->type, p, ctx->num_sms, st));
+    return KD_ATTN_OK;
+}
+
+kd_attn_status rms_norm_fp8_core(kd_attn_ctx* ctx, const kd_tensor* x, const kd_tensor* residual, const float* gain,
+                                 float eps, kd_tensor* h, kd_fp8_rows* out, cudaStream_t st) {
+    kd_attn_status rc;
+    Norm8Params p{};
+    TokenRows tx, tr, th;
+    if ((rc = check_fp8_rows(ctx, out, "out", &p.out))) return rc;
+    if (p.out.K > kNorm8MaxCols)
+        return fail(ctx, KD_ATTN_ERR_UNSUPPORTED, "rows of %d columns: at most %d", p.out.K, kNorm8MaxCols);
+    if (!(eps >= 0.0f) || std::isinf(eps)) return fail(ctx, KD_ATTN_ERR_INVALID_ARGUMENT, "eps is not a number >= 0");
+    if ((rc = check_token_rows(ctx, x, "x", p.out.K, p.out.rows, false, &tx))) return rc;
+    if (residual && (rc = check_token_rows(ctx, residual, "residual", p.out.K, p.out.rows, false, &tr))) return rc;
+    if (h && (rc = check_token_rows(ctx, h, "h", p.out.K, p.out.rows, true, &th))) return rc;
+    for (const kd_tensor* t : {residual, static_cast<const kd_tensor*>(h)})
+        if (t && (t->type != x->type || t->ne[1] != x->ne[1] || t->ne[2] != x->ne[2]))
+            return fail(ctx, KD_ATTN_ERR_INVALID_ARGUMENT, "residual and h must have the type and sizes of x");
+    if (reinterpret_cast<uintptr_t>(gain) % 4) return fail(ctx, KD_ATTN_ERR_UNSUPPORTED, "gain is not 4-byte aligned");
+    p.x = x->data;
+    p.x_nb1 = tx.nb1;
+    p.x_nb2 = tx.nb2;
+    p.x_vec = tx.vec;
+    // rows are addressed as (sequence, token) unless every tensor's are evenly spaced
+    p.L = x->ne[1] > 0 ? x->ne[1] : 1;
+    if (tx.L == p.out.rows && (!residual || tr.L == p.out.rows) && (!h || th.L == p.out.rows) && p.out.rows > 0)
+        p.L = p.out.rows;
+    if (residual) {
+        p.r = residual->data;
+        p.r_nb1 = tr.nb1;
+        p.r_nb2 = tr.nb2;
+        p.r_vec = tr.vec;
+    }
+    if (h) {
+        p.h = h->data;
+        p.h_nb1 = th.nb1;
+        p.h_nb2 = th.nb2;
+        p.h_vec = th.vec;
+    }
+    p.gain = gain;
+    p.gain_vec = aligned16(gain);
+    p.eps = eps;
+    KD_CUDA(ctx, launch_norm8(x->type, p, st));
+    return KD_ATTN_OK;
+}
+
+// The codes of 8-bit rows as a 2-D map {K, rows}: a box of 128 columns (one 128-byte swizzled row in shared memory)
+// x box_rows; columns past K and rows past the end read as zeros.
+kd_attn_status make_fp8_map(kd_attn_ctx* ctx, CUtensorMap* map, const Fp8Rows& r, uint32_t box_rows) {
+    PFN_encodeTiled_t enc = get_encode();
+    if (!enc) return fail(ctx, KD_ATTN_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+    cuuint64_t dims[2] = {(cuuint64_t)r.K, (cuuint64_t)r.rows};
+    cuuint64_t strides[1] = {(cuuint64_t)r.row_bytes};
+    cuuint32_t box[2] = {128, box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    const CUresult e = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, r.codes, dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (e != CUDA_SUCCESS)
+        return fail(ctx, KD_ATTN_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled rejected 8-bit rows (%d)", (int)e);
+    return KD_ATTN_OK;
+}
+
+kd_attn_status linear_fp8_core(kd_attn_ctx* ctx, const kd_fp8_rows* x, const kd_fp8_rows* w, const float* bias,
+                               kd_tensor* y, cudaStream_t st) {
+    kd_attn_status rc;
+    Fp8Rows X{}, W{};
+    TokenRows ty;
+    if ((rc = check_fp8_rows(ctx, x, "x", &X)) || (rc = check_fp8_rows(ctx, w, "w", &W))) return rc;
+    if (X.K != W.K)
+        return fail(ctx, KD_ATTN_ERR_INVALID_ARGUMENT, "x has %d columns and w %d", X.K, W.K);
+    if ((rc = check_token_rows(ctx, y, "y", W.rows, X.rows, true, &ty))) return rc;
+    if (reinterpret_cast<uintptr_t>(bias) % 4) return fail(ctx, KD_ATTN_ERR_UNSUPPORTED, "bias is not 4-byte aligned");
+    if (X.rows == 0 || W.rows == 0) return KD_ATTN_OK;
+    Gemm8Params p{};
+    p.x_scales = X.scales;
+    p.w_scales = W.scales;
+    p.M = (int)X.rows;
+    p.N = (int)W.rows;
+    p.K = X.K;
+    p.ktiles = X.ktiles;
+    p.bias = bias;
+    p.y = y->data;
+    p.y_nb1 = ty.nb1;
+    p.y_nb2 = ty.nb2;
+    p.L = ty.L;
+    p.err = ctx->d_words;
+    p.wait_ns = ctx->wait_ns;
+    gemm8_plan(&p, ctx->num_sms);
+    CUtensorMap tmX, tmW;
+    if ((rc = make_fp8_map(ctx, &tmX, X, (uint32_t)p.nt)) || (rc = make_fp8_map(ctx, &tmW, W, kGemm8BoxRows)))
+        return rc;
+    KD_CUDA(ctx, launch_gemm8(out_type_of(y->type), tmX, tmW, p, st));
+    return KD_ATTN_OK;
+}
+
 // DiTSelfAttention::forward (crossdit.hpp:117-154) from the hidden states: fused QKV projection, flash
 // attention, out-projection.  Scratch: [Q][K][V operands][attention output][GEMM work, shared by both GEMMs].
 // The head dim of a block whose projections map to C features over n_head heads (DiTSelfAttention's and
@@ -1592,6 +1807,45 @@ kd_attn_status kd_attn_linear(kd_attn_ctx* ctx, const kd_tensor* x, const kd_lin
     if (!ctx) return KD_ATTN_ERR_INVALID_ARGUMENT;
     DeviceGuard g(ctx->device);
     return linear_core(ctx, x, w, y, static_cast<cudaStream_t>(stream));
+}
+
+kd_attn_status kd_attn_fp8_scale_bytes(int64_t K, int64_t rows, size_t* bytes) {
+    if (!bytes || K <= 0 || rows < 0) return KD_ATTN_ERR_INVALID_ARGUMENT;
+    if (K > kFp8MaxCols || rows > kFp8MaxRows) return KD_ATTN_ERR_UNSUPPORTED;
+    *bytes = (size_t)((rows + 127) / 128) * (size_t)fp8_ktiles(K) * 512;
+    return KD_ATTN_OK;
+}
+
+kd_attn_status kd_attn_quantize_fp8(kd_attn_ctx* ctx, const kd_tensor* x, kd_fp8_rows* out, void* stream) {
+    if (!ctx) return KD_ATTN_ERR_INVALID_ARGUMENT;
+    DeviceGuard g(ctx->device);
+    return quantize_fp8_core(ctx, x, out, static_cast<cudaStream_t>(stream));
+}
+
+kd_attn_status kd_attn_quantize_weight_fp8(kd_attn_ctx* ctx, const kd_linear* w, kd_fp8_rows* out, void* stream) {
+    if (!ctx) return KD_ATTN_ERR_INVALID_ARGUMENT;
+    DeviceGuard g(ctx->device);
+    return quantize_weight_fp8_core(ctx, w, out, static_cast<cudaStream_t>(stream));
+}
+
+kd_attn_status kd_attn_dequantize_fp8(kd_attn_ctx* ctx, const kd_fp8_rows* x, kd_tensor* y, void* stream) {
+    if (!ctx) return KD_ATTN_ERR_INVALID_ARGUMENT;
+    DeviceGuard g(ctx->device);
+    return dequantize_fp8_core(ctx, x, y, static_cast<cudaStream_t>(stream));
+}
+
+kd_attn_status kd_attn_rms_norm_fp8(kd_attn_ctx* ctx, const kd_tensor* x, const kd_tensor* residual,
+                                    const float* gain, float eps, kd_tensor* h, kd_fp8_rows* out, void* stream) {
+    if (!ctx) return KD_ATTN_ERR_INVALID_ARGUMENT;
+    DeviceGuard g(ctx->device);
+    return rms_norm_fp8_core(ctx, x, residual, gain, eps, h, out, static_cast<cudaStream_t>(stream));
+}
+
+kd_attn_status kd_attn_linear_fp8(kd_attn_ctx* ctx, const kd_fp8_rows* x, const kd_fp8_rows* w, const float* bias,
+                                  kd_tensor* y, void* stream) {
+    if (!ctx) return KD_ATTN_ERR_INVALID_ARGUMENT;
+    DeviceGuard g(ctx->device);
+    return linear_fp8_core(ctx, x, w, bias, y, static_cast<cudaStream_t>(stream));
 }
 
 kd_attn_status kd_attn_self_attention_block(kd_attn_ctx* ctx, const kd_tensor* x, const kd_linear* wq,

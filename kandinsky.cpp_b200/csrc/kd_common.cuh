@@ -318,6 +318,20 @@ __host__ __device__ constexpr uint32_t idesc_f16_f32acc(bool bf16, int M, int N,
            ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
+// Shared-memory descriptor of scale tiles for tcgen05.cp.32x128b: no swizzle, version 1, groups of 8 rows of
+// 16 bytes, 128 bytes apart (SBO; one 16-byte column, so LBO is not used).
+__host__ __device__ constexpr uint64_t desc_scale_tile(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(128u >> 4) << 32) | (1ull << 46);
+}
+
+// Instruction descriptor for tcgen05.mma kind::mxf8f6f4 with both operands e4m3 and K-major, and scales of
+// 8-bit exponents:
+//   [4,6) B scale id  [7,10) A format (0 = e4m3)  [10,13) B format  [17,23) N >> 3  [23] scale format (1 = ue8m0)
+//   [24,29) M >> 4  [29,31) A scale id; the ids pick one of the four scale bytes of a 32-bit TMEM column.
+__host__ __device__ constexpr uint32_t idesc_e4m3_block(int M, int N, uint32_t scale_id) {
+    return (scale_id << 4) | ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 4) << 24) | (scale_id << 29);
+}
+
 // ------------------------------------------------------------------ math
 // Packed pairs of f32 (sm_100 f32x2 arithmetic): one instruction for two independent
 // round-to-nearest operations, bit-identical to the two scalar ones.

@@ -182,6 +182,74 @@ cudaError_t launch_to_bf16_rows(const void* x, long long nb1, long long nb2, int
 // (cos, sin) of every token and rotary pair of the 3D RoPE table: cs[l * pairs + i], pairs = D/2.
 cudaError_t launch_rope_table(const RopeTab& tab, int L, int pairs, float2* cs, int num_sms, cudaStream_t st);
 
+// ---------------------------------------------------------------- 8-bit rows (kd_fp8.cu, kd_gemm8.cu)
+// Rows of e4m3 codes with a power-of-two scale per 128 columns, laid out as kd_fp8.cuh says.
+struct Fp8Rows {
+    uint8_t* codes;
+    long long row_bytes;  // a multiple of 16, at least Kp
+    uint8_t* scales;      // ceil(rows / 128) * ktiles tiles of 512 bytes, 16-byte aligned
+    int K, Kp;            // columns, and K rounded up to 16
+    int ktiles;           // ceil(ceil(K / 128) / 4)
+    long long rows;
+};
+struct Norm8Params {
+    const void* x;                     // [K, L, N], dim 0 contiguous
+    const void* r;                     // residual, or null
+    void* h;                           // x + residual, or null (may be x or r itself)
+    const float* gain;                 // [K] or null
+    long long x_nb1, x_nb2, r_nb1, r_nb2, h_nb1, h_nb2;
+    bool x_vec, r_vec, h_vec, gain_vec;  // 16-byte aligned base and rows
+    long long L;                       // tokens per sequence
+    float eps;
+    Fp8Rows out;                       // L * N rows
+};
+struct Quant8Params {
+    const void* x;
+    long long x_nb1, x_nb2;
+    bool x_vec;
+    long long L;
+    Fp8Rows out;
+};
+struct Dequant8Params {
+    Fp8Rows in;
+    void* y;
+    long long y_nb1, y_nb2;
+    bool y_vec;
+    long long L;
+};
+constexpr int kNorm8MaxCols = 32768;
+cudaError_t launch_norm8(int type, const Norm8Params& p, cudaStream_t st);
+cudaError_t launch_quant8(int type, const Quant8Params& p, int num_sms, cudaStream_t st);
+// q8_0 (or q4_0) weight rows row_bytes apart, 2-byte aligned; out.K a multiple of 32.
+cudaError_t launch_quant8_ggml(const void* w, bool q4, long long row_bytes, const Fp8Rows& out, int num_sms,
+                               cudaStream_t st);
+cudaError_t launch_dequant8(int type, const Dequant8Params& p, int num_sms, cudaStream_t st);
+
+// y[m][n] = sum_k x[m][k] w[n][k] + bias[n] of two 8-bit operands (kd_gemm8.cu).
+struct Gemm8Params {
+    const uint8_t* x_scales;
+    const uint8_t* w_scales;
+    int M, N, K;              // tokens, output features, input features
+    int ktiles;               // scale tiles along a row of either operand
+    int nt;                   // tokens per tile (a multiple of 16, at most 256)
+    int splits;               // CTAs of a cluster that share a tile's K range
+    const float* bias;        // [N] or null
+    void* y;                  // token m = l + L * n at y + l * y_nb1 + n * y_nb2
+    long long y_nb1, y_nb2;
+    long long L;
+    unsigned* err;
+    unsigned long long wait_ns;
+};
+// Rows of a TMA box of the weight operand; the token operand's box has Gemm8Params::nt rows.
+constexpr int kGemm8BoxRows = 128;
+constexpr int kGemm8MaxTokens = 256;
+// Token tile and K split of a product (the rule is explained at its definition).
+void gemm8_plan(Gemm8Params* p, int num_sms);
+// tmX / tmW: e4m3 rows as 2-D maps {K, rows} with {128, nt} and {128, kGemm8BoxRows} boxes, 128-byte swizzled, zero
+// fill past K and past the last row.
+cudaError_t launch_gemm8(OutType ot, const CUtensorMap& tmX, const CUtensorMap& tmW, const Gemm8Params& p,
+                         cudaStream_t st);
+
 // One bounded wait that nothing releases (sets the self-test error bit after wait_ns).
 cudaError_t launch_wait_selftest(unsigned* err, unsigned* abort_flag, unsigned long long wait_ns, cudaStream_t st);
 

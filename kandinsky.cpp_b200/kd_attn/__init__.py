@@ -46,6 +46,8 @@ EXPORTED = [
     "kd_attn_selftest_wait", "kd_attn_noalloc_status", "kd_attn_noalloc_selftest_wait",
     "kd_attn_qkv_projection", "kd_attn_linear", "kd_attn_self_attention_block", "kd_attn_cross_attention_block",
     "kd_attn_self_attention_block_sharded",
+    "kd_attn_fp8_scale_bytes", "kd_attn_quantize_fp8", "kd_attn_quantize_weight_fp8", "kd_attn_dequantize_fp8",
+    "kd_attn_rms_norm_fp8", "kd_attn_linear_fp8",
 ]
 
 # scratch held by the allocation-free entry point on each device (KD_ATTN_NOALLOC_SCRATCH_BYTES)
@@ -106,6 +108,40 @@ class KdLinear(ctypes.Structure):
         return w
 
 
+class _Fp8RowsStruct(ctypes.Structure):
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("ne", ctypes.c_int64 * 2),
+                ("nb1", ctypes.c_size_t)]
+
+
+class Fp8Rows:
+    """kd_fp8_rows: rows of e4m3 codes with a power-of-two scale per 128 columns, an operand of ``linear_fp8``.
+
+    codes: device tensor (rows, at least in_features rounded up to 16) of float8_e4m3fn or uint8, its rows a
+    multiple of 16 bytes apart; scales: device uint8 tensor of ``fp8_scale_bytes(in_features, rows)`` bytes, in the
+    tile order kd_attn.h gives.  The object keeps both tensors alive."""
+
+    def __init__(self, codes, scales, in_features):
+        if codes.dim() != 2 or codes.element_size() != 1 or codes.stride(1) != 1:
+            raise ValueError("codes must be a 2-D tensor of bytes with contiguous rows")
+        rows, K = codes.shape[0], int(in_features)
+        if codes.shape[1] < (K + 15) // 16 * 16:
+            raise ValueError("codes must have in_features columns, rounded up to 16")
+        if scales.element_size() != 1 or not scales.is_contiguous() or scales.numel() < fp8_scale_bytes(K, rows):
+            raise ValueError("scales must be contiguous bytes, fp8_scale_bytes(in_features, rows) of them")
+        if codes.device != scales.device:
+            raise ValueError("codes and scales must be on one device")
+        self.codes, self.scales, self.rows, self.in_features = codes, scales, rows, K
+        self.struct = _Fp8RowsStruct(codes.data_ptr(), scales.data_ptr(), (K, rows), codes.stride(0))
+
+    @staticmethod
+    def empty(rows, in_features, device="cuda"):
+        """Buffers for rows x in_features; code rows are padded to 128 bytes."""
+        import torch
+        codes = torch.empty(rows, (int(in_features) + 127) // 128 * 128, dtype=torch.uint8, device=device)
+        scales = torch.zeros(fp8_scale_bytes(in_features, rows), dtype=torch.uint8, device=device)
+        return Fp8Rows(codes.view(torch.float8_e4m3fn), scales, in_features)
+
+
 class Rope3D(ctypes.Structure):
     """kd_rope3d: 3D (t,h,w) RoPE of rope.hpp:56-102, computed on the fly."""
     _fields_ = [("axes_dim", ctypes.c_int32 * 3), ("grid", ctypes.c_int32 * 3),
@@ -159,6 +195,19 @@ def _load():
     L.kd_attn_qkv_projection.restype = st
     L.kd_attn_linear.argtypes = [P, T, W, T, P]
     L.kd_attn_linear.restype = st
+    F = ctypes.POINTER(_Fp8RowsStruct)
+    L.kd_attn_fp8_scale_bytes.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.POINTER(ctypes.c_size_t)]
+    L.kd_attn_fp8_scale_bytes.restype = st
+    L.kd_attn_quantize_fp8.argtypes = [P, T, F, P]
+    L.kd_attn_quantize_fp8.restype = st
+    L.kd_attn_quantize_weight_fp8.argtypes = [P, W, F, P]
+    L.kd_attn_quantize_weight_fp8.restype = st
+    L.kd_attn_dequantize_fp8.argtypes = [P, F, T, P]
+    L.kd_attn_dequantize_fp8.restype = st
+    L.kd_attn_rms_norm_fp8.argtypes = [P, T, T, P, ctypes.c_float, T, F, P]
+    L.kd_attn_rms_norm_fp8.restype = st
+    L.kd_attn_linear_fp8.argtypes = [P, F, F, P, T, P]
+    L.kd_attn_linear_fp8.restype = st
     L.kd_attn_self_attention_block.argtypes = [P, T, W, W, W, W, ctypes.c_int32, P, P, ctypes.c_float,
                                                ctypes.POINTER(Rope3D), T, P]
     L.kd_attn_self_attention_block.restype = st
@@ -238,6 +287,15 @@ def tile_bitmap(keep):
     import numpy as np
     keep = np.asarray(keep, dtype=bool)
     return np.packbits(keep, axis=1, bitorder="little")
+
+
+def fp8_scale_bytes(in_features, rows):
+    """Bytes of the scale tiles of 8-bit rows."""
+    n = ctypes.c_size_t()
+    rc = lib.kd_attn_fp8_scale_bytes(int(in_features), int(rows), ctypes.byref(n))
+    if rc != OK:
+        raise KdAttnError(rc, f"8-bit rows of {in_features} columns x {rows} rows")
+    return n.value
 
 
 def nccl_unique_id() -> bytes:
@@ -366,6 +424,36 @@ class Context:
     def linear(self, x, w, y, stream=None):
         """ops::linear: y (N, L, C) = x (N, L, K) W^T + b; x f32 or bf16, w a KdLinear, y f32/bf16/f16."""
         self.check(lib.kd_attn_linear(self.handle, _ref(x), ctypes.byref(w), _ref(y), _stream_ptr(stream)))
+        return y
+
+    def quantize_fp8(self, x, out, stream=None):
+        """x (N, L, K), (L, K) or (K,) f32/f16/bf16 into the 8-bit rows out (an Fp8Rows of N * L rows)."""
+        self.check(lib.kd_attn_quantize_fp8(self.handle, _ref(x), ctypes.byref(out.struct), _stream_ptr(stream)))
+        return out
+
+    def quantize_weight_fp8(self, w, out, stream=None):
+        """The weight of a KdLinear into 8-bit rows, laid out once for ``linear_fp8``; its bias is not read."""
+        self.check(lib.kd_attn_quantize_weight_fp8(self.handle, ctypes.byref(w), ctypes.byref(out.struct),
+                                                   _stream_ptr(stream)))
+        return out
+
+    def dequantize_fp8(self, x, y, stream=None):
+        """The values of the 8-bit rows x into y (N, L, K) f32/f16/bf16."""
+        self.check(lib.kd_attn_dequantize_fp8(self.handle, ctypes.byref(x.struct), _ref(y), _stream_ptr(stream)))
+        return y
+
+    def rms_norm_fp8(self, x, out, residual=None, gain=None, eps=1e-6, h=None, stream=None):
+        """s = x + residual (rounded to x's type, into h when given), out = s / sqrt(mean(s^2) + eps) * gain in 8
+        bits.  x, residual, h (N, L, K) of one type f32/f16/bf16; gain f32 (K,) or None; h may be x or residual."""
+        self.check(lib.kd_attn_rms_norm_fp8(self.handle, _ref(x), _ref(residual), _ptr(gain), float(eps), _ref(h),
+                                            ctypes.byref(out.struct), _stream_ptr(stream)))
+        return out
+
+    def linear_fp8(self, x, w, y, bias=None, stream=None):
+        """ops::linear on 8-bit operands: y (N, L, C) f32/bf16/f16 = x W^T + b; x an Fp8Rows of N * L rows, w an
+        Fp8Rows of C rows, bias f32 (C,) or None."""
+        self.check(lib.kd_attn_linear_fp8(self.handle, ctypes.byref(x.struct), ctypes.byref(w.struct), _ptr(bias),
+                                          _ref(y), _stream_ptr(stream)))
         return y
 
     def self_attention_block(self, x, wq, wk, wv, wo, n_head, y, q_gain=None, k_gain=None, eps=1e-6, rope=None,
