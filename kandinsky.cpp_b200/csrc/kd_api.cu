@@ -1449,6 +1449,23 @@ kd_attn_status make_fp8_map(kd_attn_ctx* ctx, CUtensorMap* map, const Fp8Rows& r
     return KD_ATTN_OK;
 }
 
+// The scale tiles of 8-bit rows as a 3-D map {128 words, tiles along a row, 128-row groups}: a box is one tile of
+// box_groups row groups; groups past the end read as zeros.
+kd_attn_status make_scale_map(kd_attn_ctx* ctx, CUtensorMap* map, const Fp8Rows& r, uint32_t box_groups) {
+    PFN_encodeTiled_t enc = get_encode();
+    if (!enc) return fail(ctx, KD_ATTN_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+    cuuint64_t dims[3] = {128, (cuuint64_t)r.ktiles, (cuuint64_t)((r.rows + 127) / 128)};
+    cuuint64_t strides[2] = {512, (cuuint64_t)r.ktiles * 512};
+    cuuint32_t box[3] = {128, 1, box_groups};
+    cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult e = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, r.scales, dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (e != CUDA_SUCCESS)
+        return fail(ctx, KD_ATTN_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled rejected the scales (%d)", (int)e);
+    return KD_ATTN_OK;
+}
+
 kd_attn_status linear_fp8_core(kd_attn_ctx* ctx, const kd_fp8_rows* x, const kd_fp8_rows* w, const float* bias,
                                kd_tensor* y, cudaStream_t st) {
     kd_attn_status rc;
@@ -1468,17 +1485,21 @@ kd_attn_status linear_fp8_core(kd_attn_ctx* ctx, const kd_fp8_rows* x, const kd_
     p.K = X.K;
     p.ktiles = X.ktiles;
     p.bias = bias;
+    p.bias_vec = aligned16(bias);
     p.y = y->data;
     p.y_nb1 = ty.nb1;
     p.y_nb2 = ty.nb2;
-    p.L = ty.L;
+    p.y_vec = ty.vec;
+    p.L = (int)ty.L;
     p.err = ctx->d_words;
     p.wait_ns = ctx->wait_ns;
     gemm8_plan(&p, ctx->num_sms);
-    CUtensorMap tmX, tmW;
-    if ((rc = make_fp8_map(ctx, &tmX, X, (uint32_t)p.nt)) || (rc = make_fp8_map(ctx, &tmW, W, kGemm8BoxRows)))
+    CUtensorMap tm[4] = {};
+    if ((rc = make_fp8_map(ctx, &tm[0], X, p.many ? 128u : (uint32_t)p.nt)) ||
+        (rc = make_fp8_map(ctx, &tm[1], W, p.many ? (uint32_t)p.nt / 2 : (uint32_t)kGemm8BoxRows)))
         return rc;
-    KD_CUDA(ctx, launch_gemm8(out_type_of(y->type), tmX, tmW, p, st));
+    if (p.many && ((rc = make_scale_map(ctx, &tm[2], X, 1)) || (rc = make_scale_map(ctx, &tm[3], W, 2)))) return rc;
+    KD_CUDA(ctx, launch_gemm8(out_type_of(y->type), tm, p, ctx->num_sms, st));
     return KD_ATTN_OK;
 }
 

@@ -89,6 +89,13 @@ __device__ __forceinline__ __half round_to<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// The output row of token m; L tokens to a sequence (all of them when the rows are evenly spaced).
+__device__ __forceinline__ char* token_row(const Gemm8Params& p, int m) {
+    char* y = static_cast<char*>(p.y);
+    if (p.L >= p.M) return y + (long long)m * p.y_nb1;
+    return y + (long long)(m / p.L) * p.y_nb2 + (long long)(m % p.L) * p.y_nb1;
+}
+
 // ------------------------------------------------------------------ few tokens
 // One CTA: 128 output features (the MMA's M) x nt tokens (its N) over a range of K blocks.  With few tokens the
 // weight's bytes are the work, so weights are the operand of full height and the tokens only widen the instruction.
@@ -217,8 +224,7 @@ __global__ void __launch_bounds__(kSThreads, 1)
                     for (int j = 0; j < 16; ++j) {
                         const int m = m0 + c + j;
                         if (m < p.M && n < p.N)
-                            *reinterpret_cast<TO*>(static_cast<char*>(p.y) + (m / p.L) * p.y_nb2 + (m % p.L) * p.y_nb1 +
-                                                   (long long)n * sizeof(TO)) = round_to<TO>(v[j] + bias);
+                            reinterpret_cast<TO*>(token_row(p, m))[n] = round_to<TO>(v[j] + bias);
                     }
                 }
             } else {
@@ -250,7 +256,7 @@ __global__ void __launch_bounds__(kSThreads, 1)
                     a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
                 }
                 const int m = m0 + c;
-                TO* y = reinterpret_cast<TO*>(static_cast<char*>(p.y) + (m / p.L) * p.y_nb2 + (m % p.L) * p.y_nb1) + n;
+                TO* y = reinterpret_cast<TO*>(token_row(p, m)) + n;
                 const float v[4] = {a.x + b[0], a.y + b[1], a.z + b[2], a.w + b[3]};
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
@@ -272,6 +278,321 @@ __global__ void __launch_bounds__(kSThreads, 1)
         tc_fence_after();
         tmem_dealloc(tmem, kSTmemCols);
     }
+}
+
+// ------------------------------------------------------------------ many tokens
+// Tiles of 256 tokens x bn features (256, 192 or 128) on CTA pairs: tcgen05.mma.cta_group::2 reads 128 token rows and
+// bn / 2 feature rows from each CTA, so an operand byte is staged once for both.  TMEM holds one accumulator (bn
+// columns) and two sets of scale columns; sixteen epilogue warps take it into registers at once and free it before
+// they store, so the next tile's MMAs wait for that load only.
+// A stage is two blocks of 128 columns: 32 KB of tokens and up to 32 KB of weights per CTA, and the scale tiles of
+// the CTA's tokens and of all the tile's features (each CTA multiplies its tokens with every feature).
+constexpr int kPairM = 256, kHalfM = 128;
+constexpr int kPStages = 3;
+constexpr int kPSubBytes = 128 * 128;                       // one block of 128 rows
+constexpr int kPStageBytes = 4 * kPSubBytes;
+constexpr int kPScaleAt = kPStages * kPStageBytes;
+constexpr int kPBarAt = kPScaleAt + kPStages * kSScaleBytes;
+constexpr int kPNumBars = 2 * kPStages + 2;                 // full, empty, accumulator full / read
+constexpr int kPSlotAt = kPBarAt + kPNumBars * 8;
+constexpr int kPSmem = kPSlotAt + 16 + 1024;
+static_assert(kPSmem <= 232448, "shared memory budget");
+constexpr int kPEpiWarps = 16, kPThreads = 32 * (kPEpiWarps + 2);  // then the copy warp and the MMA warp
+constexpr int kBandM = 8;  // token tiles swept together, so that the tiles in flight share operands in L2
+
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t saddr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// Loads into this CTA's shared memory, counted on an mbarrier of the pair's rank 0.
+__device__ __forceinline__ void tma_pair_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+        : "memory");
+}
+__device__ __forceinline__ void tma_pair_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+__device__ __forceinline__ void mma8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t sa, uint32_t sb, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred e, p;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(
+            d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+        : "memory");
+}
+// The scale tile at the same offset in both CTAs' shared memory into the same columns of both CTAs' TMEM.
+__device__ __forceinline__ void scales_to_tmem_pair(uint32_t tmem, uint64_t desc) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t}\n" ::"r"(tmem),
+        "l"(desc)
+        : "memory");
+}
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}\n" ::"r"(
+            smem_u32(bar)),
+        "h"((unsigned short)0x3)
+        : "memory");
+}
+
+// 64 consecutive columns of one row from registers: n0 is the row's first column here, N the row's length.
+template <typename TO>
+__device__ __forceinline__ void store_row64(TO* row, int n0, int N, bool vec, const float (&v)[64]) {
+    constexpr int kW = 16 / sizeof(TO);  // elements of a 16-byte store
+#pragma unroll
+    for (int i = 0; i < 64; i += kW) {
+        if (vec && n0 + i + kW <= N) {
+            if constexpr (sizeof(TO) == 4)
+                *reinterpret_cast<float4*>(row + n0 + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            else
+                *reinterpret_cast<uint4*>(row + n0 + i) =
+                    make_uint4(Pack2<TO>::pack(v[i], v[i + 1]), Pack2<TO>::pack(v[i + 2], v[i + 3]),
+                               Pack2<TO>::pack(v[i + 4], v[i + 5]), Pack2<TO>::pack(v[i + 6], v[i + 7]));
+        } else {
+#pragma unroll
+            for (int j = 0; j < kW; ++j)
+                if (n0 + i + j < N) row[n0 + i + j] = round_to<TO>(v[i + j]);
+        }
+    }
+}
+
+template <typename TO>
+__global__ void __launch_bounds__(kPThreads, 1)
+    gemm8_many_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
+                      const __grid_constant__ CUtensorMap tmXs, const __grid_constant__ CUtensorMap tmWs,
+                      const __grid_constant__ Gemm8Params p) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const uint32_t base = smem_u32(smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + kPBarAt);  // rank 0's count both CTAs' bytes
+    uint64_t* empty = full + kPStages;                             // each CTA's: its stage may be refilled
+    uint64_t* acc_full = empty + kPStages;
+    uint64_t* acc_read = acc_full + 1;                             // rank 0's: both CTAs hold the accumulator in registers
+    uint32_t* slot = reinterpret_cast<uint32_t*>(smem + kPSlotAt);
+    unsigned* abort_flag = slot + 1;
+    const DevCtl ctl{p.err, abort_flag, p.wait_ns};
+    const uint32_t rank = cluster_rank();
+    const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+    const int bn = p.nt;
+    const int m_tiles = (p.M + kPairM - 1) / kPairM, n_tiles = (p.N + bn - 1) / bn;
+    const long long tiles = (long long)m_tiles * n_tiles;
+    const int blocks = (p.K + 127) >> 7, steps = (blocks + 1) >> 1;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kPStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(acc_full, 1);
+        mbar_init(acc_read, 2 * 32 * kPEpiWarps);
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == kPEpiWarps + 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(kSTmemCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem = *slot;
+    const uint32_t full0 = map_to_rank(smem_u32(full), 0);
+    const uint32_t acc_read0 = map_to_rank(smem_u32(acc_read), 0);
+
+    auto tile_at = [&](long long t, int& mt, int& nt) {
+        const long long band = t / ((long long)kBandM * n_tiles);
+        const int first = (int)band * kBandM, gm = min(kBandM, m_tiles - first);
+        const int within = (int)(t - band * kBandM * n_tiles);
+        mt = first + within % gm;
+        nt = within / gm;
+    };
+
+    if (warp == kPEpiWarps) {
+        // ------------------------------------------------------------ copies (both CTAs)
+        uint32_t it = 0;
+        bool ok = true;
+        const uint32_t half_bytes = (uint32_t)bn * 64u;  // bn / 2 rows of 128 bytes
+        for (long long t = pair; t < tiles && ok; t += npairs) {
+            int mt, nt;
+            tile_at(t, mt, nt);
+            const int m0 = mt * kPairM + (int)rank * kHalfM, n0 = nt * bn;
+            for (int st = 0; st < steps; ++st, ++it) {
+                const int s = it % kPStages;
+                if (!(ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((it / kPStages) & 1u) ^ 1u, ctl, kErrTimeoutKVEmpty))))
+                    break;
+                if (lane == 0) {
+                    const bool scales = (st & 1) == 0;  // a scale tile covers two stages
+                    const uint32_t a = base + s * kPStageBytes, b = a + 2 * kPSubBytes, bar = full0 + 8u * s;
+                    if (rank == 0)
+                        mbar_arrive_expect_tx(&full[s], 2 * (2 * kPSubBytes + 2 * half_bytes + (scales ? kSScaleBytes : 0)));
+                    tma_pair_2d(a, &tmX, bar, st * 256, m0);
+                    tma_pair_2d(b, &tmW, bar, st * 256, n0 + (int)rank * (bn / 2));
+                    tma_pair_2d(a + kPSubBytes, &tmX, bar, st * 256 + 128, m0);
+                    tma_pair_2d(b + half_bytes, &tmW, bar, st * 256 + 128, n0 + (int)rank * (bn / 2));
+                    if (scales) {
+                        const uint32_t sc = base + kPScaleAt + s * kSScaleBytes;
+                        tma_pair_3d(sc, &tmXs, bar, 0, st >> 1, m0 >> 7);
+                        tma_pair_3d(sc + 512, &tmWs, bar, 0, st >> 1, n0 >> 7);
+                    }
+                }
+                __syncwarp();
+            }
+        }
+        // wait for the releases of the last stages: nothing may be addressed to this CTA when it leaves
+        if (ok)
+            for (uint32_t k = (it > (uint32_t)kPStages ? it - kPStages : 0u); k < it; ++k)
+                if (!__all_sync(0xffffffffu, mbar_wait(&empty[k % kPStages], (k / kPStages) & 1u, ctl, kErrTimeoutDrain)))
+                    break;
+    } else if (warp == kPEpiWarps + 1) {
+        // ------------------------------------------------------------ MMAs (rank 0)
+        if (rank == 0) {
+            constexpr uint32_t dhi = sw128_desc_hi(1024);
+            const uint32_t idesc0 = idesc_e4m3_block(kPairM, bn, 0);
+            uint32_t it = 0, tc = 0;
+            bool ok = true, issued = false;
+            for (long long t = pair; t < tiles && ok; t += npairs, ++tc) {
+                int mt, nt;
+                tile_at(t, mt, nt);
+                const uint32_t col = (uint32_t)((nt * bn) & 127) >> 5;  // the tile's first feature in its scale tile: 0 or 64
+                if (tc >= 1 &&
+                    !(ok = __all_sync(0xffffffffu, mbar_wait(acc_read, (tc - 1) & 1u, ctl, kErrTimeoutO))))
+                    break;
+                tc_fence_after();
+                for (int st = 0; st < steps; ++st, ++it) {
+                    const int s = it % kPStages;
+                    if (!(ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (it / kPStages) & 1u, ctl, kErrTimeoutKVFull))))
+                        break;
+                    tc_fence_after();
+                    const uint32_t sa = tmem + kSScaleCol + 16u * (uint32_t)((st >> 1) & 1), sb = sa + 4;
+                    if ((st & 1) == 0) {
+                        const uint32_t sc = base + kPScaleAt + s * kSScaleBytes;
+                        scales_to_tmem_pair(sa, desc_scale_tile(sc));
+                        scales_to_tmem_pair(sb, desc_scale_tile(sc + 512));
+                        scales_to_tmem_pair(sb + 4, desc_scale_tile(sc + 1024));
+                    }
+                    const uint32_t a = base + s * kPStageBytes, b = a + 2 * kPSubBytes;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (2 * st + h >= blocks) break;  // (the scale bytes of a block past the end are anything)
+                        const uint32_t id = (uint32_t)(2 * (st & 1) + h);
+                        const uint32_t idesc = idesc0 | (id << 4) | (id << 29);
+                        const uint32_t alo = sw128_desc_lo(a + h * kPSubBytes, 16);
+                        const uint32_t blo = sw128_desc_lo(b + h * (uint32_t)bn * 64u, 16);
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            mma8_pair(tmem, desc_join(alo + kk * 2, dhi), desc_join(blo + kk * 2, dhi), idesc, sa, sb + col,
+                                      (st | h | kk) ? 1u : 0u);
+                    }
+                    commit_pair(&empty[s]);
+                    issued = true;
+                }
+                if (ok) commit_pair(acc_full);
+            }
+            if (!ok && issued) {  // gave up: a further arrival once every MMA issued so far has retired
+                commit_pair(acc_full);
+                mbar_wait(acc_full, tc & 1u, ctl, kErrTimeoutDrain, false);
+            }
+        }
+    } else {
+        // ------------------------------------------------------------ epilogue: bias, rounding, stores
+        const int r = ((warp & 3) << 5) + lane, g = warp >> 2;  // token row of this CTA, columns 64 g .. of the tile
+        const uint32_t src = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 64u * g;
+        uint32_t tc = 0;
+        for (long long t = pair; t < tiles; t += npairs, ++tc) {
+            int mt, nt;
+            tile_at(t, mt, nt);
+            if (!__all_sync(0xffffffffu, mbar_wait(acc_full, tc & 1u, ctl, kErrTimeoutO))) break;
+            tc_fence_after();
+            float v[64];
+            if (64 * g < bn) {
+                uint32_t u[64];
+                tmem_ld64_sync(src, u);
+#pragma unroll
+                for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(u[i]);
+            }
+            tc_fence_before();
+            mbar_arrive_remote(acc_read0);
+            const int m = mt * kPairM + (int)rank * kHalfM + r, n = nt * bn + 64 * g;
+            if (64 * g >= bn || n >= p.N || m >= p.M) continue;
+            if (p.bias) {
+                if (p.bias_vec && n + 64 <= p.N) {
+                    const float4* b4 = reinterpret_cast<const float4*>(p.bias + n);
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) {
+                        const float4 b = __ldg(b4 + q);
+                        v[4 * q] += b.x, v[4 * q + 1] += b.y, v[4 * q + 2] += b.z, v[4 * q + 3] += b.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 64; ++q)
+                        if (n + q < p.N) v[q] += __ldg(p.bias + n + q);
+                }
+            }
+            store_row64(reinterpret_cast<TO*>(token_row(p, m)), n, p.N, p.y_vec, v);
+        }
+    }
+    // After a wait gave up, copies may still be landing: give them time before the memory is released.
+    __syncwarp();
+    if (threadIdx.x == 0 && *reinterpret_cast<volatile unsigned*>(abort_flag)) {
+        const unsigned long long t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 50000ull) {
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync_all();  // no CTA leaves while its partner may still signal its barriers
+    if (warp == kPEpiWarps + 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kSTmemCols) : "memory");
+    }
+}
+
+template <typename TO>
+cudaError_t many_typed(const CUtensorMap* tm, const Gemm8Params& p, int num_sms, cudaStream_t st) {
+    auto kern = gemm8_many_kernel<TO>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPSmem);
+    if (e != cudaSuccess) return e;
+    const long long tiles = (long long)((p.M + kPairM - 1) / kPairM) * ((p.N + p.nt - 1) / p.nt);
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.blockDim = dim3(kPThreads);
+    cfg.dynamicSmemBytes = kPSmem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cfg.gridDim = dim3((unsigned)(2 * (num_sms / 2)));
+    // pairs that can be resident at one time; asked once, for every B200 is alike
+    static const int resident = [&] {
+        int n = 0;
+        return cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess ? n : 0;
+    }();
+    if (resident <= 0) return cudaErrorInvalidConfiguration;
+    cfg.gridDim = dim3((unsigned)(2 * (tiles < resident ? tiles : resident)));
+    return cudaLaunchKernelEx(&cfg, kern, tm[0], tm[1], tm[2], tm[3], p);
 }
 
 template <typename TO>
@@ -296,21 +617,40 @@ cudaError_t few_typed(const CUtensorMap& tmX, const CUtensorMap& tmW, const Gemm
 
 }  // namespace
 
-// Tokens per tile: all of them up to 256 (in steps of 16).  K is split while the tiles leave more than half of the
-// SMs idle and each part keeps at least two blocks, over at most 8 CTAs (the portable cluster size).
+// Few tokens (at most 256): all of them in one tile, in steps of 16; K is split while the tiles leave more than half
+// of the SMs idle and each part keeps at least two blocks, over at most 8 CTAs (the portable cluster size).
+// Many tokens: the tile width whose rounds over the SM pairs cost least, counting a tile's columns and the fixed
+// part of a tile (measured: about 24 columns' worth).
 void gemm8_plan(Gemm8Params* p, int num_sms) {
-    p->nt = p->M >= kGemm8MaxTokens ? kGemm8MaxTokens : (p->M + 15) / 16 * 16;
-    const long long tiles = (long long)((p->N + kGemm8BoxRows - 1) / kGemm8BoxRows) * ((p->M + p->nt - 1) / p->nt);
-    const int blocks = (p->K + 127) / 128;
     p->splits = 1;
-    while (p->splits < 8 && tiles * p->splits * 2 <= num_sms && blocks >= p->splits * 4) p->splits *= 2;
+    p->many = p->M > kGemm8MaxTokens;
+    if (!p->many) {
+        p->nt = (p->M + 15) / 16 * 16;
+        const long long tiles = (p->N + kGemm8BoxRows - 1) / kGemm8BoxRows;
+        const int blocks = (p->K + 127) / 128;
+        while (p->splits < 8 && tiles * p->splits * 2 <= num_sms && blocks >= p->splits * 4) p->splits *= 2;
+        return;
+    }
+    const long long m_tiles = (p->M + kPairM - 1) / kPairM, pairs = num_sms / 2;
+    long long best = -1;
+    for (const int bn : {256, 192, 128}) {
+        const long long tiles = m_tiles * ((p->N + bn - 1) / bn);
+        const long long cost = (tiles + pairs - 1) / pairs * (bn + 24);
+        if (best < 0 || cost < best) {
+            best = cost;
+            p->nt = bn;
+        }
+    }
 }
 
-cudaError_t launch_gemm8(OutType ot, const CUtensorMap& tmX, const CUtensorMap& tmW, const Gemm8Params& p,
-                         cudaStream_t st) {
-    return ot == OutType::F32 ? few_typed<float>(tmX, tmW, p, st)
-                              : (ot == OutType::F16 ? few_typed<__half>(tmX, tmW, p, st)
-                                                    : few_typed<__nv_bfloat16>(tmX, tmW, p, st));
+cudaError_t launch_gemm8(OutType ot, const CUtensorMap* tm, const Gemm8Params& p, int num_sms, cudaStream_t st) {
+    if (p.many)
+        return ot == OutType::F32 ? many_typed<float>(tm, p, num_sms, st)
+                                  : (ot == OutType::F16 ? many_typed<__half>(tm, p, num_sms, st)
+                                                        : many_typed<__nv_bfloat16>(tm, p, num_sms, st));
+    return ot == OutType::F32 ? few_typed<float>(tm[0], tm[1], p, st)
+                              : (ot == OutType::F16 ? few_typed<__half>(tm[0], tm[1], p, st)
+                                                    : few_typed<__nv_bfloat16>(tm[0], tm[1], p, st));
 }
 
 }  // namespace kd

@@ -231,24 +231,25 @@ struct Gemm8Params {
     const uint8_t* w_scales;
     int M, N, K;              // tokens, output features, input features
     int ktiles;               // scale tiles along a row of either operand
-    int nt;                   // tokens per tile (a multiple of 16, at most 256)
-    int splits;               // CTAs of a cluster that share a tile's K range
+    bool many;                // more than kGemm8MaxTokens tokens: CTA pairs
+    int nt;                   // few tokens: tokens of the tile (a multiple of 16); many: features per tile
+    int splits;               // few tokens: CTAs of a cluster that share a tile's K range
     const float* bias;        // [N] or null
+    bool bias_vec, y_vec;     // 16-byte aligned bias; output rows
     void* y;                  // token m = l + L * n at y + l * y_nb1 + n * y_nb2
     long long y_nb1, y_nb2;
-    long long L;
+    int L;                    // at least M when the rows are evenly spaced (y_nb2 is not read)
     unsigned* err;
     unsigned long long wait_ns;
 };
-// Rows of a TMA box of the weight operand; the token operand's box has Gemm8Params::nt rows.
 constexpr int kGemm8BoxRows = 128;
 constexpr int kGemm8MaxTokens = 256;
-// Token tile and K split of a product (the rule is explained at its definition).
+// Chooses the kernel and its tile (the rule is explained at its definition).
 void gemm8_plan(Gemm8Params* p, int num_sms);
-// tmX / tmW: e4m3 rows as 2-D maps {K, rows} with {128, nt} and {128, kGemm8BoxRows} boxes, 128-byte swizzled, zero
-// fill past K and past the last row.
-cudaError_t launch_gemm8(OutType ot, const CUtensorMap& tmX, const CUtensorMap& tmW, const Gemm8Params& p,
-                         cudaStream_t st);
+// tm[0], tm[1]: the codes of x and w as 2-D maps {K, rows}, 128-byte swizzled, zero fill; boxes of 128 columns x
+// nt (few) or 128 (many) rows of x and 128 (few) or nt / 2 (many) rows of w.  many: tm[2], tm[3]: the scale tiles of x
+// and w as 3-D maps {128 words, ktiles, ceil(rows / 128)} with {128, 1, 1} and {128, 1, 2} boxes.
+cudaError_t launch_gemm8(OutType ot, const CUtensorMap* tm, const Gemm8Params& p, int num_sms, cudaStream_t st);
 
 // One bounded wait that nothing releases (sets the self-test error bit after wait_ns).
 cudaError_t launch_wait_selftest(unsigned* err, unsigned* abort_flag, unsigned long long wait_ns, cudaStream_t st);

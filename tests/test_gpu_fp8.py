@@ -232,7 +232,7 @@ def check_product(y, x64, w64, bias, dtype, label=""):
 
 SIZES = [(1, 1, 1), (1, 128, 128), (2, 130, 16), (1, 1000, 4096), (16, 256, 512), (17, 100, 200), (33, 129, 640),
          (77, 384, 1000), (128, 128, 1152), (129, 384, 520), (256, 200, 2048), (257, 300, 640), (600, 520, 1792),
-         (1030, 256, 130)]
+         (1030, 256, 130), (3000, 1152, 300), (4608, 1000, 520)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
