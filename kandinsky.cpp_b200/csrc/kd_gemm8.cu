@@ -446,10 +446,15 @@ __global__ void __launch_bounds__(kPThreads, 1)
                     const uint32_t a = base + s * kPStageBytes, b = a + 2 * kPSubBytes, bar = full0 + 8u * s;
                     if (rank == 0)
                         mbar_arrive_expect_tx(&full[s], 2 * (2 * kPSubBytes + 2 * half_bytes + (scales ? kSScaleBytes : 0)));
-                    tma_pair_2d(a, &tmX, bar, st * 256, m0);
-                    tma_pair_2d(b, &tmW, bar, st * 256, n0 + (int)rank * (bn / 2));
-                    tma_pair_2d(a + kPSubBytes, &tmX, bar, st * 256 + 128, m0);
-                    tma_pair_2d(b + half_bytes, &tmW, bar, st * 256 + 128, n0 + (int)rank * (bn / 2));
+                    if (p.whole_blocks) {
+                        tma_pair_3d(a, &tmX, bar, 0, m0, 2 * st);
+                        tma_pair_3d(b, &tmW, bar, 0, n0 + (int)rank * (bn / 2), 2 * st);
+                    } else {
+                        tma_pair_2d(a, &tmX, bar, st * 256, m0);
+                        tma_pair_2d(b, &tmW, bar, st * 256, n0 + (int)rank * (bn / 2));
+                        tma_pair_2d(a + kPSubBytes, &tmX, bar, st * 256 + 128, m0);
+                        tma_pair_2d(b + half_bytes, &tmW, bar, st * 256 + 128, n0 + (int)rank * (bn / 2));
+                    }
                     if (scales) {
                         const uint32_t sc = base + kPScaleAt + s * kSScaleBytes;
                         tma_pair_3d(sc, &tmXs, bar, 0, st >> 1, m0 >> 7);
@@ -624,6 +629,7 @@ cudaError_t few_typed(const CUtensorMap& tmX, const CUtensorMap& tmW, const Gemm
 void gemm8_plan(Gemm8Params* p, int num_sms) {
     p->splits = 1;
     p->many = p->M > kGemm8MaxTokens;
+    p->whole_blocks = p->many && p->K % 128 == 0;
     if (!p->many) {
         p->nt = (p->M + 15) / 16 * 16;
         const long long tiles = (p->N + kGemm8BoxRows - 1) / kGemm8BoxRows;

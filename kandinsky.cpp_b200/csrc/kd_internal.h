@@ -232,6 +232,7 @@ struct Gemm8Params {
     int M, N, K;              // tokens, output features, input features
     int ktiles;               // scale tiles along a row of either operand
     bool many;                // more than kGemm8MaxTokens tokens: CTA pairs
+    bool whole_blocks;        // many tokens and K a multiple of 128: maps by blocks (below)
     int nt;                   // few tokens: tokens of the tile (a multiple of 16); many: features per tile
     int splits;               // few tokens: CTAs of a cluster that share a tile's K range
     const float* bias;        // [N] or null
@@ -247,7 +248,8 @@ constexpr int kGemm8MaxTokens = 256;
 // Chooses the kernel and its tile (the rule is explained at its definition).
 void gemm8_plan(Gemm8Params* p, int num_sms);
 // tm[0], tm[1]: the codes of x and w as 2-D maps {K, rows}, 128-byte swizzled, zero fill; boxes of 128 columns x
-// nt (few) or 128 (many) rows of x and 128 (few) or nt / 2 (many) rows of w.  many: tm[2], tm[3]: the scale tiles of x
+// nt (few) or 128 (many) rows of x and 128 (few) or nt / 2 (many) rows of w; whole_blocks: 3-D maps {128,
+// rows, K / 128} whose boxes bring two blocks.  many: tm[2], tm[3]: the scale tiles of x
 // and w as 3-D maps {128 words, ktiles, ceil(rows / 128)} with {128, 1, 1} and {128, 1, 2} boxes.
 cudaError_t launch_gemm8(OutType ot, const CUtensorMap* tm, const Gemm8Params& p, int num_sms, cudaStream_t st);
 
