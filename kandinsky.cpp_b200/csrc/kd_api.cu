@@ -1490,7 +1490,7 @@ kd_attn_status linear_fp8_core(kd_attn_ctx* ctx, const kd_fp8_rows* x, const kd_
     p.y = y->data;
     p.y_nb1 = ty.nb1;
     p.y_nb2 = ty.nb2;
-    p.y_vec = ty.vec;
+    p.y_vec = reinterpret_cast<uintptr_t>(y->data) % 32 == 0 && ty.nb1 % 32 == 0 && ty.nb2 % 32 == 0;
     p.L = (int)ty.L;
     p.err = ctx->d_words;
     p.wait_ns = ctx->wait_ns;

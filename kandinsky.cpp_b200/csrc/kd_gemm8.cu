@@ -353,19 +353,27 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar) {
         : "memory");
 }
 
-// 64 consecutive columns of one row from registers: n0 is the row's first column here, N the row's length.
+// 32 bytes in one store: a whole sector, where two 16-byte stores reach L2 as two partial writes.
+__device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&u)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(u[0]), "r"(u[1]), "r"(u[2]),
+                 "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+                 : "memory");
+}
+// 64 consecutive columns of one row from registers: n0 is the row's first column here, N the row's length; vec: the
+// rows start on 32-byte boundaries.
 template <typename TO>
 __device__ __forceinline__ void store_row64(TO* row, int n0, int N, bool vec, const float (&v)[64]) {
-    constexpr int kW = 16 / sizeof(TO);  // elements of a 16-byte store
+    constexpr int kW = 32 / sizeof(TO);  // elements of a 32-byte store
 #pragma unroll
     for (int i = 0; i < 64; i += kW) {
         if (vec && n0 + i + kW <= N) {
-            if constexpr (sizeof(TO) == 4)
-                *reinterpret_cast<float4*>(row + n0 + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-            else
-                *reinterpret_cast<uint4*>(row + n0 + i) =
-                    make_uint4(Pack2<TO>::pack(v[i], v[i + 1]), Pack2<TO>::pack(v[i + 2], v[i + 3]),
-                               Pack2<TO>::pack(v[i + 4], v[i + 5]), Pack2<TO>::pack(v[i + 6], v[i + 7]));
+            uint32_t u[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if constexpr (sizeof(TO) == 4) u[j] = __float_as_uint(v[i + j]);
+                else u[j] = Pack2<TO>::pack(v[i + 2 * j], v[i + 2 * j + 1]);
+            }
+            st_global_v8(row + n0 + i, u);
         } else {
 #pragma unroll
             for (int j = 0; j < kW; ++j)
@@ -403,7 +411,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
             mbar_init(&empty[s], 1);
         }
         mbar_init(acc_full, 1);
-        mbar_init(acc_read, 2 * 32 * kPEpiWarps);
+        mbar_init(acc_read, 2 * kPEpiWarps);
         *abort_flag = 0;
         fence_mbar_init();
     }
@@ -537,7 +545,8 @@ __global__ void __launch_bounds__(kPThreads, 1)
                 for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(u[i]);
             }
             tc_fence_before();
-            mbar_arrive_remote(acc_read0);
+            __syncwarp();
+            if (lane == 0) mbar_arrive_remote(acc_read0);
             const int m = mt * kPairM + (int)rank * kHalfM + r, n = nt * bn + 64 * g;
             if (64 * g >= bn || n >= p.N || m >= p.M) continue;
             if (p.bias) {

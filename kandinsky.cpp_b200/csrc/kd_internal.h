@@ -236,7 +236,7 @@ struct Gemm8Params {
     int nt;                   // few tokens: tokens of the tile (a multiple of 16); many: features per tile
     int splits;               // few tokens: CTAs of a cluster that share a tile's K range
     const float* bias;        // [N] or null
-    bool bias_vec, y_vec;     // 16-byte aligned bias; output rows
+    bool bias_vec, y_vec;     // 16-byte aligned bias; 32-byte aligned output rows
     void* y;                  // token m = l + L * n at y + l * y_nb1 + n * y_nb2
     long long y_nb1, y_nb2;
     int L;                    // at least M when the rows are evenly spaced (y_nb2 is not read)
