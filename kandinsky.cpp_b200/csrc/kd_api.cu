@@ -1433,16 +1433,15 @@ kd_attn_status rms_norm_fp8_core(kd_attn_ctx* ctx, const kd_tensor* x, const kd_
 }
 
 // The codes of 8-bit rows as a 2-D map {K, rows}: a box of 128 columns (one 128-byte swizzled row in shared memory)
-// x box_rows; columns past K and rows past the end read as zeros.  by_blocks (K a multiple of 128): a 3-D map {128,
-// rows, K / 128} whose box brings two blocks of 128 columns.
-kd_attn_status make_fp8_map(kd_attn_ctx* ctx, CUtensorMap* map, const Fp8Rows& r, uint32_t box_rows, bool by_blocks) {
+// x box_rows; columns past K and rows past the end read as zeros.
+kd_attn_status make_fp8_map(kd_attn_ctx* ctx, CUtensorMap* map, const Fp8Rows& r, uint32_t box_rows) {
     PFN_encodeTiled_t enc = get_encode();
     if (!enc) return fail(ctx, KD_ATTN_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
-    cuuint64_t dims[3] = {(cuuint64_t)(by_blocks ? 128 : r.K), (cuuint64_t)r.rows, (cuuint64_t)(r.K / 128)};
-    cuuint64_t strides[2] = {(cuuint64_t)r.row_bytes, 128};
-    cuuint32_t box[3] = {128, box_rows, 2};
-    cuuint32_t estr[3] = {1, 1, 1};
-    const CUresult e = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, by_blocks ? 3 : 2, r.codes, dims, strides, box, estr,
+    cuuint64_t dims[2] = {(cuuint64_t)r.K, (cuuint64_t)r.rows};
+    cuuint64_t strides[1] = {(cuuint64_t)r.row_bytes};
+    cuuint32_t box[2] = {128, box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    const CUresult e = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, r.codes, dims, strides, box, estr,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (e != CUDA_SUCCESS)
@@ -1486,7 +1485,6 @@ kd_attn_status linear_fp8_core(kd_attn_ctx* ctx, const kd_fp8_rows* x, const kd_
     p.K = X.K;
     p.ktiles = X.ktiles;
     p.bias = bias;
-    p.bias_vec = aligned16(bias);
     p.y = y->data;
     p.y_nb1 = ty.nb1;
     p.y_nb2 = ty.nb2;
@@ -1496,10 +1494,10 @@ kd_attn_status linear_fp8_core(kd_attn_ctx* ctx, const kd_fp8_rows* x, const kd_
     p.wait_ns = ctx->wait_ns;
     gemm8_plan(&p, ctx->num_sms);
     CUtensorMap tm[4] = {};
-    if ((rc = make_fp8_map(ctx, &tm[0], X, p.many ? 128u : (uint32_t)p.nt, p.whole_blocks)) ||
-        (rc = make_fp8_map(ctx, &tm[1], W, p.many ? (uint32_t)p.nt / 2 : (uint32_t)kGemm8BoxRows, p.whole_blocks)))
+    if ((rc = make_fp8_map(ctx, &tm[0], X, p.many ? 128u : (uint32_t)p.nt)) ||
+        (rc = make_fp8_map(ctx, &tm[1], W, p.many ? (uint32_t)p.nt / 2 : (uint32_t)kGemm8BoxRows)))
         return rc;
-    if (p.many && ((rc = make_scale_map(ctx, &tm[2], X, 1)) || (rc = make_scale_map(ctx, &tm[3], W, 2)))) return rc;
+    if (p.many && ((rc = make_scale_map(ctx, &tm[2], X, 1)) || (rc = make_scale_map(ctx, &tm[3], W, (uint32_t)p.parts + 1)))) return rc;
     KD_CUDA(ctx, launch_gemm8(out_type_of(y->type), tm, p, ctx->num_sms, st));
     return KD_ATTN_OK;
 }

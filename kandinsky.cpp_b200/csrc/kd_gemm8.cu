@@ -281,23 +281,33 @@ __global__ void __launch_bounds__(kSThreads, 1)
 }
 
 // ------------------------------------------------------------------ many tokens
-// Tiles of 256 tokens x bn features (256, 192 or 128) on CTA pairs: tcgen05.mma.cta_group::2 reads 128 token rows and
-// bn / 2 feature rows from each CTA, so an operand byte is staged once for both.  TMEM holds one accumulator (bn
-// columns) and two sets of scale columns; sixteen epilogue warps take it into registers at once and free it before
-// they store, so the next tile's MMAs wait for that load only.
-// A stage is two blocks of 128 columns: 32 KB of tokens and up to 32 KB of weights per CTA, and the scale tiles of
-// the CTA's tokens and of all the tile's features (each CTA multiplies its tokens with every feature).
+// Tiles of 256 tokens on CTA pairs: tcgen05.mma.cta_group::2 reads 128 token rows and half of the feature rows from
+// each CTA, so an operand byte is staged once for both.  A tile has one or two parts of pn features (two of 192, or
+// one of 192 or 128), each an accumulator of its own in TMEM.
+//
+// What decides the shape, in cycles per block of 128 columns (B200, 31,744 x 4,096 x 4,096):
+//   - the SM takes in at most about 58 bytes a cycle from L2 (copies alone, at any copy size): 256 x 256 tiles
+//     stage 32 KB a block, 563 cycles against 512 of MMAs; 256 x 384 stage 40 KB, 706 against 768.
+//   - MMAs with N = 192 run at the full rate, with N = 128 at 0.7 of it (the tokens' rows are read again too often).
+//   - an accumulator is read out in some 1,500 cycles, and with one of 256 columns beside the scales there is no room
+//     for another: the tensor cores paused 3,800 cycles a tile.  Two parts are read out one after the other instead:
+//     at a tile's end the first part's last MMAs go first, and are read out under the second's.
 constexpr int kPairM = 256, kHalfM = 128;
-constexpr int kPStages = 3;
-constexpr int kPSubBytes = 128 * 128;                       // one block of 128 rows
-constexpr int kPStageBytes = 4 * kPSubBytes;
-constexpr int kPScaleAt = kPStages * kPStageBytes;
-constexpr int kPBarAt = kPScaleAt + kPStages * kSScaleBytes;
-constexpr int kPNumBars = 2 * kPStages + 2;                 // full, empty, accumulator full / read
+constexpr int kPTokenBytes = kHalfM * 128;                  // a stage is one block of 128 columns
+constexpr int kPRingBytes = 5 * (kPTokenBytes + 192 * 128);  // five stages of the widest tile (more of a narrower one)
+constexpr int kPMaxStages = 7;
+constexpr int kPScaleBytes = 4 * 512;                       // a stage's scale tiles: of the tokens, of 384 features
+constexpr int kPScaleAt = kPRingBytes;
+constexpr int kPBiasAt = kPScaleAt + kPMaxStages * kPScaleBytes;
+constexpr int kPBarAt = kPBiasAt + 2 * 192 * 4;
+constexpr int kPNumBars = 2 * kPMaxStages + 5;              // full, empty, two accumulators' full and read, drain
 constexpr int kPSlotAt = kPBarAt + kPNumBars * 8;
 constexpr int kPSmem = kPSlotAt + 16 + 1024;
 static_assert(kPSmem <= 232448, "shared memory budget");
-constexpr int kPEpiWarps = 16, kPThreads = 32 * (kPEpiWarps + 2);  // then the copy warp and the MMA warp
+// Two groups of eight epilogue warps, one for each accumulator, then the copy warp and the MMA warp.
+constexpr int kPGroupWarps = 8, kPEpiWarps = 16, kPThreads = 32 * (kPEpiWarps + 2);
+constexpr uint32_t kPAccCols = 192;
+constexpr uint32_t kPScaleCol = 384;  // two sets: 4 columns of the tokens, 12 of the features
 constexpr int kBandM = 8;  // token tiles swept together, so that the tiles in flight share operands in L2
 
 __device__ __forceinline__ uint32_t map_to_rank(uint32_t saddr, uint32_t rank) {
@@ -323,13 +333,22 @@ __device__ __forceinline__ void tma_pair_3d(uint32_t dst, const CUtensorMap* map
         "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
         : "memory");
 }
-__device__ __forceinline__ void mma8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                          uint32_t sa, uint32_t sb, uint32_t accumulate) {
+// The four MMAs of a block of 128 columns (32 bytes of each operand row apart), issued by one lane.  One warp issues
+// all MMAs of a pair, so its instructions count: with an election and a descriptor for each MMA, and the ring's and
+// the parts' bookkeeping at run time, the loop took 1,700 cycles a block where the MMAs take 768.
+__device__ __forceinline__ void mma8_pair_block(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                                uint32_t sa, uint32_t sb, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred e, p;\n\t"
+        "{\n\t.reg .pred e, p, t;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
         "elect.sync _|e, 0xffffffff;\n\t"
         "setp.ne.b32 p, %6, 0;\n\t"
-        "@e tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(
+        "setp.eq.b32 t, 0, 0;\n\t"
+        "add.s64 a1, %1, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 a3, %1, 6;\n\t"
+        "add.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a1, b1, %3, [%4], [%5], t;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a2, b2, %3, [%4], [%5], t;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a3, b3, %3, [%4], [%5], t;\n\t}\n" ::"r"(
             d_tmem),
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
         : "memory");
@@ -354,35 +373,34 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar) {
 }
 
 // 32 bytes in one store: a whole sector, where two 16-byte stores reach L2 as two partial writes.
-__device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&u)[8]) {
+__device__ __forceinline__ void st_global_v8(void* p, const uint32_t* u) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(u[0]), "r"(u[1]), "r"(u[2]),
                  "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
                  : "memory");
 }
-// 64 consecutive columns of one row from registers: n0 is the row's first column here, N the row's length; vec: the
-// rows start on 32-byte boundaries.
+// 32 consecutive columns of one row, rounded already (two to a word in 16 bits): n0 is the row's first column here, N
+// the row's length; vec: the rows start on 32-byte boundaries.
 template <typename TO>
-__device__ __forceinline__ void store_row64(TO* row, int n0, int N, bool vec, const float (&v)[64]) {
+__device__ __forceinline__ void store_row32(TO* row, int n0, int N, bool vec, const uint32_t* u) {
     constexpr int kW = 32 / sizeof(TO);  // elements of a 32-byte store
 #pragma unroll
-    for (int i = 0; i < 64; i += kW) {
-        if (vec && n0 + i + kW <= N) {
-            uint32_t u[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if constexpr (sizeof(TO) == 4) u[j] = __float_as_uint(v[i + j]);
-                else u[j] = Pack2<TO>::pack(v[i + 2 * j], v[i + 2 * j + 1]);
-            }
-            st_global_v8(row + n0 + i, u);
+    for (int i = 0; i < 32 / kW; ++i) {
+        if (vec && n0 + (i + 1) * kW <= N) {
+            st_global_v8(row + n0 + i * kW, u + 8 * i);
         } else {
 #pragma unroll
-            for (int j = 0; j < kW; ++j)
-                if (n0 + i + j < N) row[n0 + i + j] = round_to<TO>(v[i + j]);
+            for (int j = 0; j < kW; ++j) {
+                if (n0 + i * kW + j >= N) break;
+                if constexpr (sizeof(TO) == 4)
+                    reinterpret_cast<uint32_t*>(row)[n0 + i * kW + j] = u[8 * i + j];
+                else
+                    reinterpret_cast<uint16_t*>(row)[n0 + i * kW + j] = (uint16_t)(u[8 * i + (j >> 1)] >> (16 * (j & 1)));
+            }
         }
     }
 }
 
-template <typename TO>
+template <typename TO, int kParts>
 __global__ void __launch_bounds__(kPThreads, 1)
     gemm8_many_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                       const __grid_constant__ CUtensorMap tmXs, const __grid_constant__ CUtensorMap tmWs,
@@ -392,26 +410,33 @@ __global__ void __launch_bounds__(kPThreads, 1)
     const uint32_t base = smem_u32(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + kPBarAt);  // rank 0's count both CTAs' bytes
-    uint64_t* empty = full + kPStages;                             // each CTA's: its stage may be refilled
-    uint64_t* acc_full = empty + kPStages;
-    uint64_t* acc_read = acc_full + 1;                             // rank 0's: both CTAs hold the accumulator in registers
+    uint64_t* empty = full + kPMaxStages;                          // each CTA's: its stage may be refilled
+    uint64_t* acc_full = empty + kPMaxStages;                      // [2]
+    uint64_t* acc_read = acc_full + 2;                             // [2], rank 0's: both CTAs have read the accumulator
+    uint64_t* drain = acc_read + 2;
     uint32_t* slot = reinterpret_cast<uint32_t*>(smem + kPSlotAt);
     unsigned* abort_flag = slot + 1;
     const DevCtl ctl{p.err, abort_flag, p.wait_ns};
     const uint32_t rank = cluster_rank();
     const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
-    const int bn = p.nt;
+    const int pn = p.nt, bn = pn * kParts;
     const int m_tiles = (p.M + kPairM - 1) / kPairM, n_tiles = (p.N + bn - 1) / bn;
     const long long tiles = (long long)m_tiles * n_tiles;
-    const int blocks = (p.K + 127) >> 7, steps = (blocks + 1) >> 1;
+    const int blocks = (p.K + 127) >> 7;
+    const uint32_t part_bytes = (uint32_t)pn * 64u;  // pn / 2 feature rows of 128 bytes
+    const uint32_t stage_bytes = kPTokenBytes + (uint32_t)kParts * part_bytes;
+    const uint32_t stages = min((uint32_t)kPRingBytes / stage_bytes, (uint32_t)kPMaxStages);
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kPStages; ++s) {
+        for (int s = 0; s < kPMaxStages; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
-        mbar_init(acc_full, 1);
-        mbar_init(acc_read, 2 * kPEpiWarps);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&acc_full[i], 1);
+            mbar_init(&acc_read[i], 2 * kPGroupWarps);
+        }
+        mbar_init(drain, 1);
         *abort_flag = 0;
         fence_mbar_init();
     }
@@ -438,132 +463,196 @@ __global__ void __launch_bounds__(kPThreads, 1)
 
     if (warp == kPEpiWarps) {
         // ------------------------------------------------------------ copies (both CTAs)
-        uint32_t it = 0;
+        constexpr uint32_t scale_bytes = 512u * (kParts + 2);
+        uint32_t s = 0, turn = 0, total = 0;
         bool ok = true;
-        const uint32_t half_bytes = (uint32_t)bn * 64u;  // bn / 2 rows of 128 bytes
         for (long long t = pair; t < tiles && ok; t += npairs) {
             int mt, nt;
             tile_at(t, mt, nt);
             const int m0 = mt * kPairM + (int)rank * kHalfM, n0 = nt * bn;
-            for (int st = 0; st < steps; ++st, ++it) {
-                const int s = it % kPStages;
-                if (!(ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((it / kPStages) & 1u) ^ 1u, ctl, kErrTimeoutKVEmpty))))
-                    break;
+            for (int kb = 0; kb < blocks; ++kb, ++total) {
+                if (!(ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], (turn & 1u) ^ 1u, ctl, kErrTimeoutKVEmpty)))) break;
                 if (lane == 0) {
-                    const bool scales = (st & 1) == 0;  // a scale tile covers two stages
-                    const uint32_t a = base + s * kPStageBytes, b = a + 2 * kPSubBytes, bar = full0 + 8u * s;
-                    if (rank == 0)
-                        mbar_arrive_expect_tx(&full[s], 2 * (2 * kPSubBytes + 2 * half_bytes + (scales ? kSScaleBytes : 0)));
-                    if (p.whole_blocks) {
-                        tma_pair_3d(a, &tmX, bar, 0, m0, 2 * st);
-                        tma_pair_3d(b, &tmW, bar, 0, n0 + (int)rank * (bn / 2), 2 * st);
-                    } else {
-                        tma_pair_2d(a, &tmX, bar, st * 256, m0);
-                        tma_pair_2d(b, &tmW, bar, st * 256, n0 + (int)rank * (bn / 2));
-                        tma_pair_2d(a + kPSubBytes, &tmX, bar, st * 256 + 128, m0);
-                        tma_pair_2d(b + half_bytes, &tmW, bar, st * 256 + 128, n0 + (int)rank * (bn / 2));
-                    }
+                    const bool scales = (kb & 3) == 0;  // a scale tile covers four blocks
+                    const uint32_t a = base + s * stage_bytes, bar = full0 + 8u * s;
+                    if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * (stage_bytes + (scales ? scale_bytes : 0u)));
+                    tma_pair_2d(a, &tmX, bar, kb * 128, m0);
+#pragma unroll
+                    for (int h = 0; h < kParts; ++h)
+                        tma_pair_2d(a + kPTokenBytes + h * part_bytes, &tmW, bar, kb * 128, n0 + h * pn + (int)rank * (pn / 2));
                     if (scales) {
-                        const uint32_t sc = base + kPScaleAt + s * kSScaleBytes;
-                        tma_pair_3d(sc, &tmXs, bar, 0, st >> 1, m0 >> 7);
-                        tma_pair_3d(sc + 512, &tmWs, bar, 0, st >> 1, n0 >> 7);
+                        const uint32_t sc = base + kPScaleAt + s * kPScaleBytes;
+                        tma_pair_3d(sc, &tmXs, bar, 0, kb >> 2, m0 >> 7);
+                        tma_pair_3d(sc + 512, &tmWs, bar, 0, kb >> 2, n0 >> 7);
                     }
                 }
                 __syncwarp();
+                if (++s == stages) s = 0, ++turn;
             }
         }
         // wait for the releases of the last stages: nothing may be addressed to this CTA when it leaves
-        if (ok)
-            for (uint32_t k = (it > (uint32_t)kPStages ? it - kPStages : 0u); k < it; ++k)
-                if (!__all_sync(0xffffffffu, mbar_wait(&empty[k % kPStages], (k / kPStages) & 1u, ctl, kErrTimeoutDrain)))
-                    break;
+        for (uint32_t k = 0; ok && k < min(total, stages); ++k) {
+            if (s == 0) s = stages, --turn;
+            --s;
+            ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], turn & 1u, ctl, kErrTimeoutDrain));
+        }
     } else if (warp == kPEpiWarps + 1) {
         // ------------------------------------------------------------ MMAs (rank 0)
         if (rank == 0) {
             constexpr uint32_t dhi = sw128_desc_hi(1024);
-            const uint32_t idesc0 = idesc_e4m3_block(kPairM, bn, 0);
-            uint32_t it = 0, tc = 0;
+            constexpr uint32_t kNextId = (1u << 4) | (1u << 29);  // the next scale byte of both operands
+            const uint32_t idesc0 = idesc_e4m3_block(kPairM, pn, 0);
+            const uint32_t lo0 = sw128_desc_lo(base, 16), lo_step = stage_bytes >> 4, part_lo = part_bytes >> 4;
+            // a part's first feature within the copied tiles, in columns of 32 features (even: multiples of 64)
+            const uint32_t part_col = (uint32_t)pn / 32u;
+            uint32_t s = 0, turn = 0, lo = lo0;            // the ring's next stage: its index, turn and descriptor word
+            uint32_t sa = tmem + kPScaleCol;               // the scale set in use; the two differ in bit 4
+            uint32_t reads = 0;                            // tiles whose accumulators (two parts) / tile (one) went out
             bool ok = true, issued = false;
-            for (long long t = pair; t < tiles && ok; t += npairs, ++tc) {
-                int mt, nt;
-                tile_at(t, mt, nt);
-                const uint32_t col = (uint32_t)((nt * bn) & 127) >> 5;  // the tile's first feature in its scale tile: 0 or 64
-                if (tc >= 1 &&
-                    !(ok = __all_sync(0xffffffffu, mbar_wait(acc_read, (tc - 1) & 1u, ctl, kErrTimeoutO))))
-                    break;
+            // Waits for the next stage and copies its scales, when it brings some.
+            auto take = [&](int i) {
+                if (!__all_sync(0xffffffffu, mbar_wait(&full[s], turn & 1u, ctl, kErrTimeoutKVFull))) return false;
                 tc_fence_after();
-                for (int st = 0; st < steps; ++st, ++it) {
-                    const int s = it % kPStages;
-                    if (!(ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (it / kPStages) & 1u, ctl, kErrTimeoutKVFull))))
+                if ((i & 3) == 0) {
+                    sa ^= 16u;
+                    const uint32_t sc = base + kPScaleAt + s * kPScaleBytes;
+#pragma unroll
+                    for (int j = 0; j < 2 + kParts; ++j) scales_to_tmem_pair(sa + 4 * j, desc_scale_tile(sc + 512 * j));
+                }
+                return true;
+            };
+            auto advance = [&] {
+                lo += lo_step;
+                if (++s == stages) s = 0, ++turn, lo = lo0;
+            };
+            auto part = [&](int i, int h, uint32_t acc, uint32_t stage_lo, uint32_t set, uint32_t col) {
+                mma8_pair_block(tmem + acc * kPAccCols, desc_join(stage_lo, dhi),
+                                desc_join(stage_lo + (kPTokenBytes >> 4) + h * part_lo, dhi), idesc0 + (uint32_t)(i & 3) * kNextId,
+                                set, set + 4 + col + h * part_col, i ? 1u : 0u);
+            };
+            // Two blocks from i (or one, at the end of a short row), the first part of both before the second's.
+            auto part_by_part = [&](int i, int n, bool first, bool last) {
+                const uint32_t s0 = s, set0 = sa ^ ((i & 3) == 0 ? 16u : 0u), l0 = lo;
+                if (!take(i)) return false;
+                part(i, 0, 0, l0, set0, 0);
+                issued = true;
+                advance();
+                const uint32_t s1 = s, l1 = lo;
+                if (n == 2) {
+                    if (!take(i + 1)) return false;
+                    part(i + 1, 0, 0, l1, sa, 0);
+                    advance();
+                }
+                if (last) commit_pair(&acc_full[0]);
+                if (first && reads) {
+                    if (!__all_sync(0xffffffffu, mbar_wait(&acc_read[1], (reads - 1) & 1u, ctl, kErrTimeoutO))) return false;
+                    tc_fence_after();
+                }
+                part(i, 1, 1, l0, set0, 0);
+                commit_pair(&empty[s0]);
+                if (n == 2) {
+                    part(i + 1, 1, 1, l1, sa, 0);
+                    commit_pair(&empty[s1]);
+                }
+                if (last) commit_pair(&acc_full[1]);
+                return true;
+            };
+            for (long long t = pair; t < tiles && ok; t += npairs, ++reads) {
+                if constexpr (kParts == 2) {
+                    if (reads && !(ok = __all_sync(0xffffffffu, mbar_wait(&acc_read[0], (reads - 1) & 1u, ctl, kErrTimeoutO))))
                         break;
                     tc_fence_after();
-                    const uint32_t sa = tmem + kSScaleCol + 16u * (uint32_t)((st >> 1) & 1), sb = sa + 4;
-                    if ((st & 1) == 0) {
-                        const uint32_t sc = base + kPScaleAt + s * kSScaleBytes;
-                        scales_to_tmem_pair(sa, desc_scale_tile(sc));
-                        scales_to_tmem_pair(sb, desc_scale_tile(sc + 512));
-                        scales_to_tmem_pair(sb + 4, desc_scale_tile(sc + 1024));
+                    if (!(ok = part_by_part(0, min(blocks, 2), true, blocks <= 2))) break;
+                    if (blocks == 3) ok = part_by_part(2, 1, false, true);
+                    if (blocks <= 3) continue;
+                    for (int i = 2; i < blocks - 2; ++i) {
+                        if (!(ok = take(i))) break;
+                        part(i, 0, 0, lo, sa, 0);
+                        part(i, 1, 1, lo, sa, 0);
+                        commit_pair(&empty[s]);
+                        advance();
                     }
-                    const uint32_t a = base + s * kPStageBytes, b = a + 2 * kPSubBytes;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (2 * st + h >= blocks) break;  // (the scale bytes of a block past the end are anything)
-                        const uint32_t id = (uint32_t)(2 * (st & 1) + h);
-                        const uint32_t idesc = idesc0 | (id << 4) | (id << 29);
-                        const uint32_t alo = sw128_desc_lo(a + h * kPSubBytes, 16);
-                        const uint32_t blo = sw128_desc_lo(b + h * (uint32_t)bn * 64u, 16);
-#pragma unroll
-                        for (int kk = 0; kk < 4; ++kk)
-                            mma8_pair(tmem, desc_join(alo + kk * 2, dhi), desc_join(blo + kk * 2, dhi), idesc, sa, sb + col,
-                                      (st | h | kk) ? 1u : 0u);
+                    ok = ok && part_by_part(blocks - 2, 2, false, true);
+                } else {
+                    int mt, nt;
+                    tile_at(t, mt, nt);
+                    const uint32_t col = (uint32_t)((nt * bn) & 127) / 32u, acc = reads & 1u;
+                    if (reads >= 2 &&
+                        !(ok = __all_sync(0xffffffffu, mbar_wait(&acc_read[acc], ((reads >> 1) - 1) & 1u, ctl, kErrTimeoutO))))
+                        break;
+                    tc_fence_after();
+                    for (int i = 0; i < blocks; ++i) {
+                        if (!(ok = take(i))) break;
+                        part(i, 0, acc, lo, sa, col);
+                        issued = true;
+                        commit_pair(&empty[s]);
+                        advance();
                     }
-                    commit_pair(&empty[s]);
-                    issued = true;
+                    if (ok) commit_pair(&acc_full[acc]);
                 }
-                if (ok) commit_pair(acc_full);
             }
-            if (!ok && issued) {  // gave up: a further arrival once every MMA issued so far has retired
-                commit_pair(acc_full);
-                mbar_wait(acc_full, tc & 1u, ctl, kErrTimeoutDrain, false);
+            if (!ok && issued) {  // gave up: wait until every MMA issued so far has retired
+                commit_pair(drain);
+                mbar_wait(drain, 0, ctl, kErrTimeoutDrain, false);
             }
         }
     } else {
         // ------------------------------------------------------------ epilogue: bias, rounding, stores
-        const int r = ((warp & 3) << 5) + lane, g = warp >> 2;  // token row of this CTA, columns 64 g .. of the tile
-        const uint32_t src = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 64u * g;
-        uint32_t tc = 0;
+        const int g = warp / kPGroupWarps;                // the accumulator of this group
+        const int r = ((warp & 3) << 5) + lane;           // token row of this CTA's 128
+        const int half = (warp >> 2) & 1, wc = pn / 2;    // columns half * wc .. of the part
+        const uint32_t src = tmem + ((uint32_t)((warp & 3) * 32) << 16) + g * kPAccCols + (uint32_t)(half * wc);
+        float* bias = reinterpret_cast<float*>(smem + kPBiasAt) + g * 192;
+        uint32_t uses = 0, tc = 0;
         for (long long t = pair; t < tiles; t += npairs, ++tc) {
+            if (kParts == 1 && (int)(tc & 1u) != g) continue;
             int mt, nt;
             tile_at(t, mt, nt);
-            if (!__all_sync(0xffffffffu, mbar_wait(acc_full, tc & 1u, ctl, kErrTimeoutO))) break;
+            const int np = nt * bn + (kParts == 2 ? g * pn : 0);  // the part's first feature
+            {  // its bias, while the MMAs run
+                const int i = threadIdx.x - g * (32 * kPGroupWarps);
+                if (uses) named_bar_sync(1 + g, 32 * kPGroupWarps);
+                if (i < pn) bias[i] = p.bias && np + i < p.N ? __ldg(p.bias + np + i) : 0.0f;
+                named_bar_sync(1 + g, 32 * kPGroupWarps);
+            }
+            // After a wait gave up the group still goes through its tiles, without waiting again: its warps meet at the
+            // named barrier, so none may leave alone.
+            const bool ok = __all_sync(0xffffffffu, *reinterpret_cast<volatile unsigned*>(abort_flag) == 0 &&
+                                                        mbar_wait(&acc_full[g], uses & 1u, ctl, kErrTimeoutO));
             tc_fence_after();
-            float v[64];
-            if (64 * g < bn) {
-                uint32_t u[64];
-                tmem_ld64_sync(src, u);
+            ++uses;
+            constexpr int kWords = sizeof(TO) == 4 ? 32 : 16;
+            uint32_t u[3 * kWords];
+            if (ok) {
 #pragma unroll
-                for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(u[i]);
+                for (int c = 0; c < 3; ++c) {
+                    if (32 * c < wc) {
+                        uint32_t x[32];
+                        tmem_ld32_sync(src + 32 * c, x);
+                        const float* b = bias + half * wc + 32 * c;
+                        if constexpr (sizeof(TO) == 4) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) u[c * kWords + j] = __float_as_uint(__uint_as_float(x[j]) + b[j]);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j)
+                                u[c * kWords + j] = Pack2<TO>::pack(__uint_as_float(x[2 * j]) + b[2 * j],
+                                                                    __uint_as_float(x[2 * j + 1]) + b[2 * j + 1]);
+                        }
+                    }
+                }
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_remote(acc_read0);
-            const int m = mt * kPairM + (int)rank * kHalfM + r, n = nt * bn + 64 * g;
-            if (64 * g >= bn || n >= p.N || m >= p.M) continue;
-            if (p.bias) {
-                if (p.bias_vec && n + 64 <= p.N) {
-                    const float4* b4 = reinterpret_cast<const float4*>(p.bias + n);
+            if (lane == 0) mbar_arrive_remote(acc_read0 + 8u * g);
+            const int m = mt * kPairM + (int)rank * kHalfM + r, n = np + half * wc;
+            if (ok && m < p.M) {
+                TO* row = reinterpret_cast<TO*>(token_row(p, m));
 #pragma unroll
-                    for (int q = 0; q < 16; ++q) {
-                        const float4 b = __ldg(b4 + q);
-                        v[4 * q] += b.x, v[4 * q + 1] += b.y, v[4 * q + 2] += b.z, v[4 * q + 3] += b.w;
-                    }
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 64; ++q)
-                        if (n + q < p.N) v[q] += __ldg(p.bias + n + q);
-                }
+                for (int c = 0; c < 3; ++c)
+                    if (32 * c < wc && n + 32 * c < p.N) store_row32(row, n + 32 * c, p.N, p.y_vec, u + c * kWords);
             }
-            store_row64(reinterpret_cast<TO*>(token_row(p, m)), n, p.N, p.y_vec, v);
+            __syncwarp();
         }
     }
     // After a wait gave up, copies may still be landing: give them time before the memory is released.
@@ -582,12 +671,12 @@ __global__ void __launch_bounds__(kPThreads, 1)
     }
 }
 
-template <typename TO>
+template <typename TO, int kParts>
 cudaError_t many_typed(const CUtensorMap* tm, const Gemm8Params& p, int num_sms, cudaStream_t st) {
-    auto kern = gemm8_many_kernel<TO>;
+    auto kern = gemm8_many_kernel<TO, kParts>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPSmem);
     if (e != cudaSuccess) return e;
-    const long long tiles = (long long)((p.M + kPairM - 1) / kPairM) * ((p.N + p.nt - 1) / p.nt);
+    const long long tiles = (long long)((p.M + kPairM - 1) / kPairM) * ((p.N + p.nt * p.parts - 1) / (p.nt * p.parts));
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -633,36 +722,40 @@ cudaError_t few_typed(const CUtensorMap& tmX, const CUtensorMap& tmW, const Gemm
 
 // Few tokens (at most 256): all of them in one tile, in steps of 16; K is split while the tiles leave more than half
 // of the SMs idle and each part keeps at least two blocks, over at most 8 CTAs (the portable cluster size).
-// Many tokens: the tile width whose rounds over the SM pairs cost least, counting a tile's columns and the fixed
-// part of a tile (measured: about 24 columns' worth).
+// Many tokens: the tile whose rounds over the SM pairs take the fewest cycles, by the cost of a block of 128 columns
+// (MMAs for two parts of 192, copies for one of 192 or 128, as measured above) and about 1,000 cycles a tile.
 void gemm8_plan(Gemm8Params* p, int num_sms) {
-    p->splits = 1;
+    p->splits = p->parts = 1;
     p->many = p->M > kGemm8MaxTokens;
-    p->whole_blocks = p->many && p->K % 128 == 0;
+    const int blocks = (p->K + 127) / 128;
     if (!p->many) {
         p->nt = (p->M + 15) / 16 * 16;
         const long long tiles = (p->N + kGemm8BoxRows - 1) / kGemm8BoxRows;
-        const int blocks = (p->K + 127) / 128;
         while (p->splits < 8 && tiles * p->splits * 2 <= num_sms && blocks >= p->splits * 4) p->splits *= 2;
         return;
     }
+    const struct { int parts, pn, block_cycles; } shapes[] = {{2, 192, 768}, {1, 192, 494}, {1, 128, 424}};
     const long long m_tiles = (p->M + kPairM - 1) / kPairM, pairs = num_sms / 2;
     long long best = -1;
-    for (const int bn : {256, 192, 128}) {
-        const long long tiles = m_tiles * ((p->N + bn - 1) / bn);
-        const long long cost = (tiles + pairs - 1) / pairs * (bn + 24);
+    for (const auto& s : shapes) {
+        const long long tiles = m_tiles * ((p->N + s.parts * s.pn - 1) / (s.parts * s.pn));
+        const long long cost = (tiles + pairs - 1) / pairs * ((long long)blocks * s.block_cycles + 1000);
         if (best < 0 || cost < best) {
             best = cost;
-            p->nt = bn;
+            p->parts = s.parts;
+            p->nt = s.pn;
         }
     }
 }
 
 cudaError_t launch_gemm8(OutType ot, const CUtensorMap* tm, const Gemm8Params& p, int num_sms, cudaStream_t st) {
     if (p.many)
-        return ot == OutType::F32 ? many_typed<float>(tm, p, num_sms, st)
-                                  : (ot == OutType::F16 ? many_typed<__half>(tm, p, num_sms, st)
-                                                        : many_typed<__nv_bfloat16>(tm, p, num_sms, st));
+        return p.parts == 2 ? (ot == OutType::F32 ? many_typed<float, 2>(tm, p, num_sms, st)
+                                                  : (ot == OutType::F16 ? many_typed<__half, 2>(tm, p, num_sms, st)
+                                                                        : many_typed<__nv_bfloat16, 2>(tm, p, num_sms, st)))
+                            : (ot == OutType::F32 ? many_typed<float, 1>(tm, p, num_sms, st)
+                                                  : (ot == OutType::F16 ? many_typed<__half, 1>(tm, p, num_sms, st)
+                                                                        : many_typed<__nv_bfloat16, 1>(tm, p, num_sms, st)));
     return ot == OutType::F32 ? few_typed<float>(tm[0], tm[1], p, st)
                               : (ot == OutType::F16 ? few_typed<__half>(tm[0], tm[1], p, st)
                                                     : few_typed<__nv_bfloat16>(tm[0], tm[1], p, st));

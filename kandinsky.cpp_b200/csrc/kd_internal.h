@@ -232,11 +232,11 @@ struct Gemm8Params {
     int M, N, K;              // tokens, output features, input features
     int ktiles;               // scale tiles along a row of either operand
     bool many;                // more than kGemm8MaxTokens tokens: CTA pairs
-    bool whole_blocks;        // many tokens and K a multiple of 128: maps by blocks (below)
-    int nt;                   // few tokens: tokens of the tile (a multiple of 16); many: features per tile
+    int nt;                   // few tokens: tokens of the tile (a multiple of 16); many: features of a part
+    int parts;                // many tokens: parts of a tile (1 or 2)
     int splits;               // few tokens: CTAs of a cluster that share a tile's K range
     const float* bias;        // [N] or null
-    bool bias_vec, y_vec;     // 16-byte aligned bias; 32-byte aligned output rows
+    bool y_vec;               // 32-byte aligned output rows
     void* y;                  // token m = l + L * n at y + l * y_nb1 + n * y_nb2
     long long y_nb1, y_nb2;
     int L;                    // at least M when the rows are evenly spaced (y_nb2 is not read)
@@ -248,9 +248,8 @@ constexpr int kGemm8MaxTokens = 256;
 // Chooses the kernel and its tile (the rule is explained at its definition).
 void gemm8_plan(Gemm8Params* p, int num_sms);
 // tm[0], tm[1]: the codes of x and w as 2-D maps {K, rows}, 128-byte swizzled, zero fill; boxes of 128 columns x
-// nt (few) or 128 (many) rows of x and 128 (few) or nt / 2 (many) rows of w; whole_blocks: 3-D maps {128,
-// rows, K / 128} whose boxes bring two blocks.  many: tm[2], tm[3]: the scale tiles of x
-// and w as 3-D maps {128 words, ktiles, ceil(rows / 128)} with {128, 1, 1} and {128, 1, 2} boxes.
+// nt (few) or 128 (many) rows of x and 128 (few) or nt / 2 (many) rows of w.  many: tm[2], tm[3]: the scale tiles of
+// x and w as 3-D maps {128 words, ktiles, ceil(rows / 128)} with boxes of 1 and parts + 1 groups of rows.
 cudaError_t launch_gemm8(OutType ot, const CUtensorMap* tm, const Gemm8Params& p, int num_sms, cudaStream_t st);
 
 // One bounded wait that nothing releases (sets the self-test error bit after wait_ns).

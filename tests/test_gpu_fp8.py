@@ -232,7 +232,9 @@ def check_product(y, x64, w64, bias, dtype, label=""):
 
 SIZES = [(1, 1, 1), (1, 128, 128), (2, 130, 16), (1, 1000, 4096), (16, 256, 512), (17, 100, 200), (33, 129, 640),
          (77, 384, 1000), (128, 128, 1152), (129, 384, 520), (256, 200, 2048), (257, 300, 640), (600, 520, 1792),
-         (1030, 256, 130), (3000, 1152, 300), (4608, 1000, 520)]
+         (1030, 256, 130), (3000, 1152, 300), (4608, 1000, 520), (4608, 1536, 640),
+         (300, 28416, 128), (20000, 384, 256), (20000, 384, 384), (9500, 1100, 96), (9500, 576, 300),
+         (20000, 256, 640)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
