@@ -1301,7 +1301,7 @@ kd_attn_status check_fp8_rows(kd_attn_ctx* ctx, const kd_fp8_rows* r, const char
 // A [K, L, N] tensor of the 8-bit path: any strides that are whole elements; `written` rows may not overlap.
 struct TokenRows {
     long long nb1 = 0, nb2 = 0, L = 1;
-    bool vec = false;  // rows start on 16-byte boundaries
+    int align = 1;  // bytes that every row starts on: 32, 16 or 1
 };
 kd_attn_status check_token_rows(kd_attn_ctx* ctx, const kd_tensor* t, const char* name, int64_t K, int64_t rows,
                                 bool written, TokenRows* out) {
@@ -1321,7 +1321,8 @@ kd_attn_status check_token_rows(kd_attn_ctx* ctx, const kd_tensor* t, const char
     out->nb2 = (long long)nb[2];
     out->L = t->ne[1] > 0 ? t->ne[1] : 1;
     if (nb[2] == nb[1] * (uint64_t)t->ne[1] || t->ne[2] == 1) out->L = rows > 0 ? rows : 1;  // evenly spaced rows
-    out->vec = aligned16(t->data) && nb[1] % 16 == 0 && nb[2] % 16 == 0;
+    const uint64_t at = reinterpret_cast<uintptr_t>(t->data) | (t->ne[1] > 1 ? nb[1] : 0) | (t->ne[2] > 1 ? nb[2] : 0);
+    out->align = at % 32 == 0 ? 32 : (at % 16 == 0 ? 16 : 1);
     return KD_ATTN_OK;
 }
 
@@ -1335,9 +1336,9 @@ kd_attn_status quantize_fp8_core(kd_attn_ctx* ctx, const kd_tensor* x, kd_fp8_ro
     p.x = x->data;
     p.x_nb1 = tx.nb1;
     p.x_nb2 = tx.nb2;
-    p.x_vec = tx.vec;
+    p.align = tx.align;
     p.L = tx.L;
-    KD_CUDA(ctx, launch_quant8(x->type, p, ctx->num_sms, st));
+    KD_CUDA(ctx, launch_quant8(x->type, p, st));
     return KD_ATTN_OK;
 }
 
@@ -1383,9 +1384,9 @@ kd_attn_status dequantize_fp8_core(kd_attn_ctx* ctx, const kd_fp8_rows* x, kd_te
     p.y = y->data;
     p.y_nb1 = ty.nb1;
     p.y_nb2 = ty.nb2;
-    p.y_vec = ty.vec;
+    p.align = ty.align;
     p.L = ty.L;
-    KD_CUDA(ctx, launch_dequant8(y->type, p, ctx->num_sms, st));
+    KD_CUDA(ctx, launch_dequant8(y->type, p, st));
     return KD_ATTN_OK;
 }
 
@@ -1408,7 +1409,7 @@ kd_attn_status rms_norm_fp8_core(kd_attn_ctx* ctx, const kd_tensor* x, const kd_
     p.x = x->data;
     p.x_nb1 = tx.nb1;
     p.x_nb2 = tx.nb2;
-    p.x_vec = tx.vec;
+    p.align = std::min({tx.align, residual ? tr.align : 32, h ? th.align : 32});
     // rows are addressed as (sequence, token) unless every tensor's are evenly spaced
     p.L = x->ne[1] > 0 ? x->ne[1] : 1;
     if (tx.L == p.out.rows && (!residual || tr.L == p.out.rows) && (!h || th.L == p.out.rows) && p.out.rows > 0)
@@ -1417,18 +1418,18 @@ kd_attn_status rms_norm_fp8_core(kd_attn_ctx* ctx, const kd_tensor* x, const kd_
         p.r = residual->data;
         p.r_nb1 = tr.nb1;
         p.r_nb2 = tr.nb2;
-        p.r_vec = tr.vec;
     }
     if (h) {
         p.h = h->data;
         p.h_nb1 = th.nb1;
         p.h_nb2 = th.nb2;
-        p.h_vec = th.vec;
     }
     p.gain = gain;
-    p.gain_vec = aligned16(gain);
+    const uintptr_t ga = reinterpret_cast<uintptr_t>(gain);
+    p.gain_align = ga % 32 == 0 ? 32 : (ga % 16 == 0 ? 16 : 1);
+    if (gain && p.gain_align < 16) p.align = 1;  // one layout of columns over the lanes for all operands
     p.eps = eps;
-    KD_CUDA(ctx, launch_norm8(x->type, p, st));
+    KD_CUDA(ctx, launch_norm8(x->type, p, ctx->num_sms, st));
     return KD_ATTN_OK;
 }
 
@@ -1488,7 +1489,7 @@ kd_attn_status linear_fp8_core(kd_attn_ctx* ctx, const kd_fp8_rows* x, const kd_
     p.y = y->data;
     p.y_nb1 = ty.nb1;
     p.y_nb2 = ty.nb2;
-    p.y_vec = reinterpret_cast<uintptr_t>(y->data) % 32 == 0 && ty.nb1 % 32 == 0 && ty.nb2 % 32 == 0;
+    p.y_vec = ty.align >= 32;
     p.L = (int)ty.L;
     p.err = ctx->d_words;
     p.wait_ns = ctx->wait_ns;

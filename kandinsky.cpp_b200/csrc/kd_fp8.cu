@@ -1,19 +1,26 @@
 // kd_fp8.cu -- writing and reading 8-bit rows (kd_fp8.cuh) on sm_100a (B200):
 //
-//   norm8_kernel      h = x + residual, v = h / sqrt(mean(h^2) + eps) * gain, v into 8-bit rows
-//   quant8_kernel     f32 / f16 / bf16 rows into 8-bit rows
+//   norm8_kernel        h = x + residual, v = h / sqrt(mean(h^2) + eps) * gain, v into 8-bit rows
+//   quant8_kernel       f32 / f16 / bf16 rows into 8-bit rows
 //   quant8_ggml_kernel  q8_0 / q4_0 weight rows into 8-bit rows
-//   dequant8_kernel   8-bit rows back to f32 / f16 / bf16
+//   dequant8_kernel     8-bit rows back to f32 / f16 / bf16
 //
 // All of them move bytes and do little else: each value is read once and written once, held in registers between.
+// A warp's unit of work is 512 columns of a row: four blocks, one 32-bit word of scale bytes, sixteen columns a lane.
+// Where rows start on 16-byte boundaries a lane holds sixteen consecutive columns and moves them in wide accesses;
+// elsewhere (odd row lengths) lane l holds columns l, l + 32, ..., so that its narrow accesses are still coalesced.
+#include <type_traits>
+
 #include "kd_fp8.cuh"
 #include "kd_internal.h"
 
 namespace kd {
 namespace {
 
-constexpr int kVec = 8;         // consecutive columns of one lane: 16 lanes are one block of 128
+constexpr int kPer = 16;        // columns of a lane
+constexpr int kChunk = 512;     // columns of a warp
 constexpr unsigned kInfBits = 0x7F800000u;
+constexpr unsigned kAll = 0xffffffffu;
 
 template <typename T>
 __device__ __forceinline__ float to_f32(T v);
@@ -32,171 +39,297 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-__device__ __forceinline__ void unpack8(const uint4& u, const __half*, float (&v)[kVec]) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
+// Sixteen values of a lane as they lie in memory (32 or 64 bytes).
+template <typename T>
+struct Raw {
+    static constexpr int kWords = sizeof(T) * kPer / 4;
+    uint32_t w[kWords];
+};
+__device__ __forceinline__ void ld_v8(const void* p, uint32_t* w) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(p)
+                 : "memory");
+}
+__device__ __forceinline__ void st_v8(void* p, const uint32_t* w) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+template <typename T>
+__device__ __forceinline__ T get(const Raw<T>& a, int j) {
+    if constexpr (sizeof(T) == 4) {
+        return __uint_as_float(a.w[j]);
+    } else {
+        const unsigned short u = (unsigned short)(a.w[j >> 1] >> (16 * (j & 1)));
+        return *reinterpret_cast<const T*>(&u);
     }
 }
-__device__ __forceinline__ void unpack8(const uint4& u, const __nv_bfloat16*, float (&v)[kVec]) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+// Even values first: of two that share a word, the even one clears it.
+template <typename T>
+__device__ __forceinline__ void put(Raw<T>& a, int j, T v) {
+    if constexpr (sizeof(T) == 4) {
+        a.w[j] = __float_as_uint(v);
+    } else {
+        const uint32_t u = *reinterpret_cast<const unsigned short*>(&v);
+        if (j & 1) a.w[j >> 1] |= u << 16;
+        else a.w[j >> 1] = u;
     }
 }
 
-// Columns c .. c+7 of a row of K, zeros at and past K.  vec: the row starts on a 16-byte boundary.
-template <typename T>
-__device__ __forceinline__ void load8(const T* row, int c, int K, bool vec, float (&v)[kVec]) {
-    if (vec && c + kVec <= K) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 a = *reinterpret_cast<const float4*>(row + c), b = *reinterpret_cast<const float4*>(row + c + 4);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+// The column of value j of a lane in the chunk from c0.
+template <bool kVec>
+__device__ __forceinline__ int column(int c0, int lane, int j) {
+    return kVec ? c0 + lane * kPer + j : c0 + j * 32 + lane;
+}
+
+// A lane's sixteen values of a row of K, zeros at and past K.  align: of the row, in bytes (32, 16 or less).
+template <typename T, bool kVec>
+__device__ __forceinline__ void load16(const T* row, int c0, int lane, int K, int align, Raw<T>& a) {
+    constexpr int kW = Raw<T>::kWords;
+    if (kVec && column<kVec>(c0, lane, kPer) <= K) {
+        const T* p = row + column<kVec>(c0, lane, 0);
+        if (align >= 32) {
+#pragma unroll
+            for (int i = 0; i < kW / 8; ++i) ld_v8(reinterpret_cast<const uint32_t*>(p) + 8 * i, a.w + 8 * i);
         } else {
-            unpack8(*reinterpret_cast<const uint4*>(row + c), row, v);
+#pragma unroll
+            for (int i = 0; i < kW / 4; ++i) {
+                const uint4 u = reinterpret_cast<const uint4*>(p)[i];
+                a.w[4 * i] = u.x, a.w[4 * i + 1] = u.y, a.w[4 * i + 2] = u.z, a.w[4 * i + 3] = u.w;
+            }
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) v[i] = c + i < K ? to_f32(row[c + i]) : 0.0f;
+        for (int i = 0; i < kW; ++i) a.w[i] = 0;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+            if (column<kVec>(c0, lane, j) < K) put(a, j, row[column<kVec>(c0, lane, j)]);
     }
 }
-template <typename T>
-__device__ __forceinline__ void store8(T* row, int c, int K, bool vec, const float (&v)[kVec]) {
-    if (vec && c + kVec <= K) {
-        if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<float4*>(row + c) = make_float4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<float4*>(row + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
+template <typename T, bool kVec>
+__device__ __forceinline__ void store16(T* row, int c0, int lane, int K, int align, const Raw<T>& a) {
+    constexpr int kW = Raw<T>::kWords;
+    if (kVec && column<kVec>(c0, lane, kPer) <= K) {
+        T* p = row + column<kVec>(c0, lane, 0);
+        if (align >= 32) {
+#pragma unroll
+            for (int i = 0; i < kW / 8; ++i) st_v8(reinterpret_cast<uint32_t*>(p) + 8 * i, a.w + 8 * i);
         } else {
-            *reinterpret_cast<uint4*>(row + c) = make_uint4(Pack2<T>::pack(v[0], v[1]), Pack2<T>::pack(v[2], v[3]),
-                                                            Pack2<T>::pack(v[4], v[5]), Pack2<T>::pack(v[6], v[7]));
+#pragma unroll
+            for (int i = 0; i < kW / 4; ++i)
+                reinterpret_cast<uint4*>(p)[i] = make_uint4(a.w[4 * i], a.w[4 * i + 1], a.w[4 * i + 2], a.w[4 * i + 3]);
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < kVec; ++i)
-            if (c + i < K) row[c + i] = from_f32<T>(v[i]);
+        for (int j = 0; j < kPer; ++j)
+            if (column<kVec>(c0, lane, j) < K) row[column<kVec>(c0, lane, j)] = get(a, j);
     }
 }
 
-// One block of 128 columns, eight to a lane of a half-warp, into codes and the block's scale byte.  Lanes at and
-// past K hold zeros.  A NaN or infinity becomes a NaN code and does not count for the scale.  Every lane of the
-// half-warp takes part; `live` lanes write.
-__device__ __forceinline__ void encode_block(const float (&v)[kVec], const Fp8Rows& o, long long row, int c,
-                                             bool live) {
-    uint32_t top = 0;
+// The largest finite magnitude (as bits) of the block of each of a lane's values: kVec: one block a lane, in top[0];
+// else block i holds values 4 i .. 4 i + 3 of every lane.  NaNs and infinities become NaN in v.
+template <bool kVec>
+__device__ __forceinline__ void block_tops(float (&v)[kPer], uint32_t (&top)[4]) {
+    constexpr int kBlocks = kVec ? 1 : 4, kIn = kPer / kBlocks;
+    bool odd = false;
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) top = max(top, __float_as_uint(fabsf(v[i])));
+    for (int b = 0; b < kBlocks; ++b) {
+        uint32_t t = 0;
 #pragma unroll
-    for (int s = 8; s; s >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, s));
-    float t[kVec];
+        for (int i = 0; i < kIn; ++i) t = max(t, __float_as_uint(fabsf(v[b * kIn + i])));
+        odd |= t >= kInfBits;
+        top[b] = t;
+    }
+    if (__any_sync(kAll, odd)) {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) t[i] = v[i];
-    // (a warp-wide vote, so that both half-warps run the shuffles of the rare path together)
-    if (__any_sync(0xffffffffu, top >= kInfBits)) {
-        top = 0;
+        for (int b = 0; b < kBlocks; ++b) {
+            uint32_t t = 0;
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-            const uint32_t a = __float_as_uint(fabsf(v[i]));
-            if (a >= kInfBits) t[i] = __uint_as_float(0x7FFFFFFFu);
-            else top = max(top, a);
+            for (int i = 0; i < kIn; ++i) {
+                const uint32_t a = __float_as_uint(fabsf(v[b * kIn + i]));
+                if (a >= kInfBits) v[b * kIn + i] = __uint_as_float(0x7FFFFFFFu);
+                else t = max(t, a);
+            }
+            top[b] = t;
         }
-#pragma unroll
-        for (int s = 8; s; s >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, s));
     }
-    const uint32_t byte = fp8_scale_byte(top);
-    if (!live) return;
-    const float inv = fp8_scale_inverse(byte);  // a power of two: the products are exact
-    const uint2 codes = make_uint2(fp8_pack4(t[0] * inv, t[1] * inv, t[2] * inv, t[3] * inv),
-                                   fp8_pack4(t[4] * inv, t[5] * inv, t[6] * inv, t[7] * inv));
-    // rows are at least K rounded up to 16 bytes long: the eight codes from c are inside when c is below that
-    if (c < o.Kp) *reinterpret_cast<uint2*>(o.codes + row * o.row_bytes + c) = codes;
-    if ((c & 127) == 0 && c < o.K) o.scales[fp8_scale_offset(row, c >> 7, o.ktiles)] = (uint8_t)byte;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+        if constexpr (kVec) {
+#pragma unroll
+            for (int s = 4; s; s >>= 1) top[b] = max(top[b], __shfl_xor_sync(kAll, top[b], s));
+        } else {
+            top[b] = __reduce_max_sync(kAll, top[b]);
+        }
+    }
 }
 
-// TPR threads hold one row, VPT vectors of eight columns each: vector j of thread t is columns 8 * (j * TPR + t).
-// One pass over the data: the row stays in registers between the sum of squares and the codes.
-template <typename T, int VPT>
-__global__ void __launch_bounds__(1024) norm8_kernel(const Norm8Params p, int tpr) {
-    __shared__ float part[32];
-    const int rows_per_cta = blockDim.x / tpr;
-    const int sub = threadIdx.x / tpr, t = threadIdx.x % tpr;
-    const long long row = (long long)blockIdx.x * rows_per_cta + sub;
-    const bool live = row < p.out.rows;
-    const long long m = live ? row : p.out.rows - 1;  // a row past the end repeats the last one and writes nothing
+// 512 columns of a row from c0, sixteen values to a lane (zeros past K), into codes and scale bytes.  All lanes take
+// part.
+template <bool kVec>
+__device__ __forceinline__ void encode16(float (&v)[kPer], const Fp8Rows& o, long long row, int c0, int lane) {
+    uint32_t top[4];
+    block_tops<kVec>(v, top);
+    uint8_t* codes = o.codes + row * o.row_bytes;
+    uint32_t word;  // the scale bytes of the four blocks
+    if constexpr (kVec) {
+        const uint32_t byte = fp8_scale_byte(top[0]);
+        word = __reduce_or_sync(kAll, byte << (8 * (lane >> 3)));
+        const float inv = fp8_scale_inverse(byte);  // a power of two: the products are exact
+        const int c = column<kVec>(c0, lane, 0);
+        if (c < o.K)  // rows are K rounded up to 16 bytes long at least
+            *reinterpret_cast<uint4*>(codes + c) =
+                make_uint4(fp8_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
+                           fp8_pack4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv),
+                           fp8_pack4(v[8] * inv, v[9] * inv, v[10] * inv, v[11] * inv),
+                           fp8_pack4(v[12] * inv, v[13] * inv, v[14] * inv, v[15] * inv));
+    } else {
+        word = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const uint32_t byte = fp8_scale_byte(top[b]);
+            word |= byte << (8 * b);
+            const float inv = fp8_scale_inverse(byte);
+            const uint32_t u = fp8_pack4(v[4 * b] * inv, v[4 * b + 1] * inv, v[4 * b + 2] * inv, v[4 * b + 3] * inv);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = column<kVec>(c0, lane, 4 * b + i);
+                if (c < o.Kp) codes[c] = (uint8_t)(u >> (8 * i));
+            }
+        }
+    }
+    uint8_t* s = o.scales + fp8_scale_offset(row, c0 >> 7, o.ktiles);
+    if (c0 + 3 * 128 < o.K) {
+        if (lane == 0) *reinterpret_cast<uint32_t*>(s) = word;
+    } else if (lane < 4 && c0 + lane * 128 < o.K) {  // bytes of blocks past K stay as they were
+        s[lane] = (uint8_t)(word >> (8 * lane));
+    }
+}
+
+// (row, 512-column chunk) of a warp's unit; 32-bit arithmetic where the units allow it.
+__device__ __forceinline__ void unit_at(long long unit, int ktiles, bool narrow, long long& row, int& chunk) {
+    if (narrow) {
+        const uint32_t u = (uint32_t)unit, r = u / (uint32_t)ktiles;
+        row = r;
+        chunk = (int)(u - r * (uint32_t)ktiles);
+    } else {
+        row = unit / ktiles;
+        chunk = (int)(unit % ktiles);
+    }
+}
+// The start of token row m, L tokens to a sequence (all of them when rows are evenly spaced).
+template <typename P>
+__device__ __forceinline__ P* row_at(P* base, long long m, long long L, long long rows, long long nb1, long long nb2) {
+    using Bytes = typename std::conditional<std::is_const<P>::value, const char, char>::type;
+    Bytes* b = reinterpret_cast<Bytes*>(base);
+    return reinterpret_cast<P*>(L >= rows ? b + m * nb1 : b + (m / L) * nb2 + (m % L) * nb1);
+}
+
+// One row at a time by blockDim.x threads (kWarpRows: by each warp of its own), thread t holding kChunks chunks of 512
+// columns from its warp's place on.  The CTA stays and takes every gridDim.x-th row: the gain is read once, and
+// the next row is on its way (in registers) while this one is summed, divided and written.  One pass over the data.
+template <typename T, bool kVec, int kChunks, bool kWarpRows>
+__global__ void __launch_bounds__(kWarpRows ? 128 : (kChunks == 1 ? 512 : 1024)) norm8_kernel(const Norm8Params p) {
+    constexpr bool kAhead = kChunks == 1;  // a second row of 32 columns a thread does not fit the registers
+    __shared__ float part[2][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int K = p.out.K;
-    const long long n = m / p.L, l = m % p.L;
-    const T* x = reinterpret_cast<const T*>(static_cast<const char*>(p.x) + n * p.x_nb2 + l * p.x_nb1);
-    const T* r = p.r ? reinterpret_cast<const T*>(static_cast<const char*>(p.r) + n * p.r_nb2 + l * p.r_nb1) : nullptr;
-    T* h = p.h ? reinterpret_cast<T*>(static_cast<char*>(p.h) + n * p.h_nb2 + l * p.h_nb1) : nullptr;
-    float v[VPT][kVec];
+    const int c0 = kWarpRows ? 0 : warp * (kChunks * kChunk);
+    const long long first = kWarpRows ? (long long)blockIdx.x * warps + warp : blockIdx.x;
+    const long long step = kWarpRows ? (long long)gridDim.x * warps : gridDim.x;
+    const long long rows = p.out.rows;
+    float g[kChunks][kPer];
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) load8(x, kVec * (j * tpr + t), K, p.x_vec, v[j]);
-    if (r) {
-        float a[VPT][kVec];
+    for (int q = 0; q < kChunks; ++q) {
+        Raw<float> a;
+        if (p.gain && kAhead) load16<float, kVec>(p.gain, c0 + q * kChunk, lane, K, p.gain_align, a);
 #pragma unroll
-        for (int j = 0; j < VPT; ++j) load8(r, kVec * (j * tpr + t), K, p.r_vec, a[j]);
-        // the sum is rounded to the rows' type, as it is stored, and the norm is of the stored value
-#pragma unroll
-        for (int j = 0; j < VPT; ++j)
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) v[j][i] = to_f32(from_f32<T>(v[j][i] + a[j][i]));
+        for (int j = 0; j < kPer; ++j) g[q][j] = p.gain && kAhead ? __uint_as_float(a.w[j]) : 1.0f;
     }
-    float sum = 0.0f;
+    auto fetch = [&](long long m, Raw<T> (&x)[kChunks], Raw<T> (&r)[kChunks]) {
+        const T* px = row_at(static_cast<const T*>(p.x), m, p.L, rows, p.x_nb1, p.x_nb2);
+        const T* pr = row_at(static_cast<const T*>(p.r), m, p.L, rows, p.r_nb1, p.r_nb2);
 #pragma unroll
-    for (int j = 0; j < VPT; ++j)
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) sum = fmaf(v[j][i], v[j][i], sum);
-    if (h && live) {
-#pragma unroll
-        for (int j = 0; j < VPT; ++j) store8(h, kVec * (j * tpr + t), K, p.h_vec, v[j]);
-    }
-#pragma unroll
-    for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-    if (tpr > 32) {
-        const int warps = tpr / 32, first = sub * warps;
-        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
-        __syncthreads();
-        sum = 0.0f;
-        for (int w = 0; w < warps; ++w) sum += part[first + w];
-    }
-    const float inv = __frcp_rn(__fsqrt_rn(__fadd_rn(__fdiv_rn(sum, (float)K), p.eps)));
-#pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-        const int c = kVec * (j * tpr + t);
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) v[j][i] *= inv;
-        if (p.gain) {
-            float g[kVec];
-            load8(p.gain, c, K, p.gain_vec, g);
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) v[j][i] *= g[i];
+        for (int q = 0; q < kChunks; ++q) {
+            load16<T, kVec>(px, c0 + q * kChunk, lane, K, p.align, x[q]);
+            if (p.r) load16<T, kVec>(pr, c0 + q * kChunk, lane, K, p.align, r[q]);
         }
-        encode_block(v[j], p.out, m, c, live);
+    };
+    Raw<T> x[kChunks], r[kChunks];
+    if (kAhead && first < rows) fetch(first, x, r);
+    int turn = 0;
+    for (long long m = first; m < rows; m += step, turn ^= 1) {
+        if (!kAhead) fetch(m, x, r);
+        float v[kChunks][kPer];
+        float sum = 0.0f;
+#pragma unroll
+        for (int q = 0; q < kChunks; ++q) {
+            if (p.r) {
+                // the sum is rounded to the rows' type, as it is stored, and the norm is of the stored value
+#pragma unroll
+                for (int j = 0; j < kPer; j += 2) {  // (a word at a time: two values of 16 bits share one)
+                    const T lo = from_f32<T>(to_f32(get(x[q], j)) + to_f32(get(r[q], j)));
+                    const T hi = from_f32<T>(to_f32(get(x[q], j + 1)) + to_f32(get(r[q], j + 1)));
+                    put(x[q], j, lo);
+                    put(x[q], j + 1, hi);
+                }
+            }
+            if (p.h) {
+                T* ph = row_at(static_cast<T*>(p.h), m, p.L, rows, p.h_nb1, p.h_nb2);
+                store16<T, kVec>(ph, c0 + q * kChunk, lane, K, p.align, x[q]);
+            }
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) {
+                v[q][j] = to_f32(get(x[q], j));
+                sum = fmaf(v[q][j], v[q][j], sum);
+            }
+        }
+        if (kAhead && m + step < rows) fetch(m + step, x, r);
+#pragma unroll
+        for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(kAll, sum, s);
+        if (!kWarpRows && warps > 1) {
+            // two buffers in turn: a warp may be one row ahead of another's reads, not two
+            if (lane == 0) part[turn][warp] = sum;
+            __syncthreads();
+            sum = lane < warps ? part[turn][lane] : 0.0f;
+#pragma unroll
+            for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(kAll, sum, s);
+        }
+        const float inv = __frcp_rn(__fsqrt_rn(__fadd_rn(__fdiv_rn(sum, (float)K), p.eps)));
+#pragma unroll
+        for (int q = 0; q < kChunks; ++q) {
+            if (!kAhead && p.gain) {
+                Raw<float> a;
+                load16<float, kVec>(p.gain, c0 + q * kChunk, lane, K, p.gain_align, a);
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) g[q][j] = __uint_as_float(a.w[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) v[q][j] = v[q][j] * inv * g[q][j];
+            if (c0 + q * kChunk < K) encode16<kVec>(v[q], p.out, m, c0 + q * kChunk, lane);
+        }
     }
 }
 
-// A half-warp per block of 128 columns.
-template <typename T>
-__global__ void quant8_kernel(const Quant8Params p) {
-    const int lane16 = threadIdx.x & 15;
-    const int blocks = (p.out.K + 127) >> 7;
-    const long long total = p.out.rows * blocks;
-    const long long step = ((long long)gridDim.x * blockDim.x) >> 4;
-    // whole warps stay in the loop: the pair's second block may be past the end
-    for (long long i = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 4; (i & ~1ll) < total; i += step) {
-        const bool live = i < total;
-        const long long row = (live ? i : total - 1) / blocks;
-        const int c = (int)((live ? i : total - 1) % blocks) * 128 + lane16 * kVec;
-        const T* x = reinterpret_cast<const T*>(static_cast<const char*>(p.x) + (row / p.L) * p.x_nb2 +
-                                                (row % p.L) * p.x_nb1);
-        float v[kVec];
-        load8(x, c, p.out.K, p.x_vec, v);
-        encode_block(v, p.out, row, c, live);
-    }
+constexpr int kUnitThreads = 256;  // eight units of a warp each
+
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(kUnitThreads) quant8_kernel(const Quant8Params p) {
+    const int lane = threadIdx.x & 31;
+    const long long unit = (long long)blockIdx.x * (kUnitThreads / 32) + (threadIdx.x >> 5);
+    const long long units = p.out.rows * p.out.ktiles;
+    if (unit >= units) return;
+    long long row;
+    int chunk;
+    unit_at(unit, p.out.ktiles, units <= 0xffffffffll, row, chunk);
+    Raw<T> a;
+    load16<T, kVec>(row_at(static_cast<const T*>(p.x), row, p.L, p.out.rows, p.x_nb1, p.x_nb2), chunk * kChunk, lane, p.out.K,
+                    p.align, a);
+    float v[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) v[j] = to_f32(get(a, j));
+    encode16<kVec>(v, p.out, row, chunk * kChunk, lane);
 }
 
 // Weight rows of 32-element ggml blocks (q8_0: f16 scale and 32 int8; q4_0: f16 scale and 16 bytes, element j in
@@ -243,7 +376,7 @@ __global__ void quant8_ggml_kernel(const uint8_t* w, int q4, long long row_bytes
             else top = max(top, a);
         }
 #pragma unroll
-        for (int s = 2; s; s >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, s));
+        for (int s = 2; s; s >>= 1) top = max(top, __shfl_xor_sync(kAll, top, s));
         const uint32_t byte = fp8_scale_byte(top);
         const float inv = fp8_scale_inverse(byte);
         if (!live || c >= o.K) continue;  // (K is a multiple of 32: a ggml block is wholly inside)
@@ -262,77 +395,111 @@ __global__ void quant8_ggml_kernel(const uint8_t* w, int q4, long long row_bytes
     }
 }
 
-// Eight codes per thread.
-template <typename T>
-__global__ void dequant8_kernel(const Dequant8Params p) {
-    const int per_row = (p.in.K + kVec - 1) / kVec;
-    const long long total = p.in.rows * per_row;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-         i += (long long)gridDim.x * blockDim.x) {
-        const long long row = i / per_row;
-        const int c = (int)(i % per_row) * kVec;
-        const uint2 u = *reinterpret_cast<const uint2*>(p.in.codes + row * p.in.row_bytes + c);
-        const float s = fp8_scale_value(p.in.scales[fp8_scale_offset(row, c >> 7, p.in.ktiles)]);
-        float a[4], b[4];
-        fp8_unpack4(u.x, a);
-        fp8_unpack4(u.y, b);
-        const float v[kVec] = {a[0] * s, a[1] * s, a[2] * s, a[3] * s, b[0] * s, b[1] * s, b[2] * s, b[3] * s};
-        T* y = reinterpret_cast<T*>(static_cast<char*>(p.y) + (row / p.L) * p.y_nb2 + (row % p.L) * p.y_nb1);
-        store8(y, c, p.in.K, p.y_vec, v);
+// Two units a warp: their loads are under way together.
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(kUnitThreads) dequant8_kernel(const Dequant8Params p) {
+    constexpr int kUnits = 2, kWarps = kUnitThreads / 32;
+    const int lane = threadIdx.x & 31;
+    const long long units = p.in.rows * p.in.ktiles;
+    const bool narrow = units <= 0xffffffffll;
+    long long row[kUnits];
+    int c0[kUnits];
+    uint32_t codes[kUnits][4], word[kUnits];
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+        const long long unit = (long long)blockIdx.x * (kWarps * kUnits) + u * kWarps + (threadIdx.x >> 5);
+        row[u] = -1;
+        if (unit >= units) continue;
+        int chunk;
+        unit_at(unit, p.in.ktiles, narrow, row[u], chunk);
+        c0[u] = chunk * kChunk;
+        const uint8_t* src = p.in.codes + row[u] * p.in.row_bytes;
+        word[u] = *reinterpret_cast<const uint32_t*>(p.in.scales + fp8_scale_offset(row[u], c0[u] >> 7, p.in.ktiles));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) codes[u][i] = 0;
+        if constexpr (kVec) {
+            if (column<kVec>(c0[u], lane, 0) < p.in.K) {  // (a code row is K rounded up to 16 bytes at least)
+                const uint4 q = *reinterpret_cast<const uint4*>(src + column<kVec>(c0[u], lane, 0));
+                codes[u][0] = q.x, codes[u][1] = q.y, codes[u][2] = q.z, codes[u][3] = q.w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < kPer; ++j)
+                if (column<kVec>(c0[u], lane, j) < p.in.K)
+                    codes[u][j >> 2] |= (uint32_t)src[column<kVec>(c0[u], lane, j)] << (8 * (j & 3));
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+        if (row[u] < 0) continue;
+        Raw<T> a;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float s = fp8_scale_value((word[u] >> (8 * (kVec ? lane >> 3 : i))) & 255u);
+            float v[4];
+            fp8_unpack4(codes[u][i], v);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) put(a, 4 * i + j, from_f32<T>(v[j] * s));
+        }
+        store16<T, kVec>(row_at(static_cast<T*>(p.y), row[u], p.L, p.in.rows, p.y_nb1, p.y_nb2), c0[u], lane, p.in.K, p.align, a);
     }
 }
 
-template <typename T>
-cudaError_t norm8_typed(const Norm8Params& p, cudaStream_t st) {
-    // up to 256 columns a warp holds a row; above, 16 (32 past 16,384) columns a thread
+// Up to 512 columns a warp has a row of its own; to 8,192 one CTA of a warp for every 512 columns; above, a warp for
+// every 1,024.  CTAs stay for as many rows as fill the GPU.
+template <typename T, bool kVec>
+cudaError_t norm8_typed(const Norm8Params& p, int num_sms, cudaStream_t st) {
     const int K = p.out.K;
-    int tpr = 32, vpt = K <= 256 ? 1 : (K <= 16384 ? 2 : 4);
-    while (tpr * vpt * kVec < K) tpr *= 2;
-    const int threads = tpr < 128 ? 128 : tpr;
-    const long long ctas = (p.out.rows + threads / tpr - 1) / (threads / tpr);
-    auto kern = vpt == 1 ? norm8_kernel<T, 1> : (vpt == 2 ? norm8_kernel<T, 2> : norm8_kernel<T, 4>);
-    kern<<<(unsigned)ctas, threads, 0, st>>>(p, tpr);
+    const bool warp_rows = K <= kChunk;
+    const int chunks = K <= 16 * kChunk ? 1 : 2;
+    const int threads = warp_rows ? 128 : (K + chunks * kChunk - 1) / (chunks * kChunk) * 32;
+    auto kern = warp_rows ? norm8_kernel<T, kVec, 1, true>
+                          : (chunks == 1 ? norm8_kernel<T, kVec, 1, false> : norm8_kernel<T, kVec, 2, false>);
+    const long long per_cta = warp_rows ? 4 : 1;
+    const long long want = (p.out.rows + per_cta - 1) / per_cta, fit = (long long)num_sms * (1024 / threads);
+    kern<<<(unsigned)(want < fit ? want : fit), threads, 0, st>>>(p);
     return cudaGetLastError();
 }
 
-unsigned grid_for(long long threads, int block, int num_sms, int per_sm) {
-    long long g = (threads + block - 1) / block;
-    const long long cap = (long long)num_sms * per_sm;
-    return (unsigned)(g > cap ? cap : (g < 1 ? 1 : g));
-}
+unsigned unit_grid(long long units, int per_cta) { return (unsigned)((units + per_cta - 1) / per_cta); }
 
 }  // namespace
 
-cudaError_t launch_norm8(int type, const Norm8Params& p, cudaStream_t st) {
+cudaError_t launch_norm8(int type, const Norm8Params& p, int num_sms, cudaStream_t st) {
     if (p.out.rows == 0) return cudaSuccess;
-    return type == 0 ? norm8_typed<float>(p, st) : (type == 1 ? norm8_typed<__half>(p, st) : norm8_typed<__nv_bfloat16>(p, st));
+    if (p.align >= 16)
+        return type == 0 ? norm8_typed<float, true>(p, num_sms, st)
+                         : (type == 1 ? norm8_typed<__half, true>(p, num_sms, st) : norm8_typed<__nv_bfloat16, true>(p, num_sms, st));
+    return type == 0 ? norm8_typed<float, false>(p, num_sms, st)
+                     : (type == 1 ? norm8_typed<__half, false>(p, num_sms, st) : norm8_typed<__nv_bfloat16, false>(p, num_sms, st));
 }
 
-cudaError_t launch_quant8(int type, const Quant8Params& p, int num_sms, cudaStream_t st) {
+cudaError_t launch_quant8(int type, const Quant8Params& p, cudaStream_t st) {
     if (p.out.rows == 0) return cudaSuccess;
-    const long long threads = p.out.rows * ((p.out.K + 127) / 128) * 16;
-    const unsigned g = grid_for(threads, 256, num_sms, 32);
-    if (type == 0) quant8_kernel<float><<<g, 256, 0, st>>>(p);
-    else if (type == 1) quant8_kernel<__half><<<g, 256, 0, st>>>(p);
-    else quant8_kernel<__nv_bfloat16><<<g, 256, 0, st>>>(p);
+    const bool vec = p.align >= 16;
+    auto kern = type == 0 ? (vec ? quant8_kernel<float, true> : quant8_kernel<float, false>)
+                          : (type == 1 ? (vec ? quant8_kernel<__half, true> : quant8_kernel<__half, false>)
+                                       : (vec ? quant8_kernel<__nv_bfloat16, true> : quant8_kernel<__nv_bfloat16, false>));
+    kern<<<unit_grid(p.out.rows * p.out.ktiles, kUnitThreads / 32), kUnitThreads, 0, st>>>(p);
     return cudaGetLastError();
 }
 
 cudaError_t launch_quant8_ggml(const void* w, bool q4, long long row_bytes, const Fp8Rows& out, int num_sms,
                                cudaStream_t st) {
     if (out.rows == 0) return cudaSuccess;
-    const long long threads = out.rows * ((out.K + 127) / 128) * 4;
-    quant8_ggml_kernel<<<grid_for(threads, 128, num_sms, 16), 128, 0, st>>>(static_cast<const uint8_t*>(w), q4 ? 1 : 0,
+    const long long ctas = (out.rows * ((out.K + 127) / 128) * 4 + 127) / 128, cap = (long long)num_sms * 16;
+    quant8_ggml_kernel<<<(unsigned)(ctas < cap ? ctas : cap), 128, 0, st>>>(static_cast<const uint8_t*>(w), q4 ? 1 : 0,
                                                                             row_bytes, out);
     return cudaGetLastError();
 }
 
-cudaError_t launch_dequant8(int type, const Dequant8Params& p, int num_sms, cudaStream_t st) {
+cudaError_t launch_dequant8(int type, const Dequant8Params& p, cudaStream_t st) {
     if (p.in.rows == 0) return cudaSuccess;
-    const unsigned g = grid_for(p.in.rows * ((p.in.K + kVec - 1) / kVec), 256, num_sms, 32);
-    if (type == 0) dequant8_kernel<float><<<g, 256, 0, st>>>(p);
-    else if (type == 1) dequant8_kernel<__half><<<g, 256, 0, st>>>(p);
-    else dequant8_kernel<__nv_bfloat16><<<g, 256, 0, st>>>(p);
+    const bool vec = p.align >= 16;
+    auto kern = type == 0 ? (vec ? dequant8_kernel<float, true> : dequant8_kernel<float, false>)
+                          : (type == 1 ? (vec ? dequant8_kernel<__half, true> : dequant8_kernel<__half, false>)
+                                       : (vec ? dequant8_kernel<__nv_bfloat16, true> : dequant8_kernel<__nv_bfloat16, false>));
+    kern<<<unit_grid(p.in.rows * p.in.ktiles, 2 * kUnitThreads / 32), kUnitThreads, 0, st>>>(p);
     return cudaGetLastError();
 }
 

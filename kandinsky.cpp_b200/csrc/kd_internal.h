@@ -198,7 +198,7 @@ struct Norm8Params {
     void* h;                           // x + residual, or null (may be x or r itself)
     const float* gain;                 // [K] or null
     long long x_nb1, x_nb2, r_nb1, r_nb2, h_nb1, h_nb2;
-    bool x_vec, r_vec, h_vec, gain_vec;  // 16-byte aligned base and rows
+    int align, gain_align;             // bytes that every row of x, r and h starts on: 32, 16, or less; gain's address
     long long L;                       // tokens per sequence
     float eps;
     Fp8Rows out;                       // L * N rows
@@ -206,7 +206,7 @@ struct Norm8Params {
 struct Quant8Params {
     const void* x;
     long long x_nb1, x_nb2;
-    bool x_vec;
+    int align;
     long long L;
     Fp8Rows out;
 };
@@ -214,16 +214,16 @@ struct Dequant8Params {
     Fp8Rows in;
     void* y;
     long long y_nb1, y_nb2;
-    bool y_vec;
+    int align;
     long long L;
 };
 constexpr int kNorm8MaxCols = 32768;
-cudaError_t launch_norm8(int type, const Norm8Params& p, cudaStream_t st);
-cudaError_t launch_quant8(int type, const Quant8Params& p, int num_sms, cudaStream_t st);
+cudaError_t launch_norm8(int type, const Norm8Params& p, int num_sms, cudaStream_t st);
+cudaError_t launch_quant8(int type, const Quant8Params& p, cudaStream_t st);
 // q8_0 (or q4_0) weight rows row_bytes apart, 2-byte aligned; out.K a multiple of 32.
 cudaError_t launch_quant8_ggml(const void* w, bool q4, long long row_bytes, const Fp8Rows& out, int num_sms,
                                cudaStream_t st);
-cudaError_t launch_dequant8(int type, const Dequant8Params& p, int num_sms, cudaStream_t st);
+cudaError_t launch_dequant8(int type, const Dequant8Params& p, cudaStream_t st);
 
 // y[m][n] = sum_k x[m][k] w[n][k] + bias[n] of two 8-bit operands (kd_gemm8.cu).
 struct Gemm8Params {
