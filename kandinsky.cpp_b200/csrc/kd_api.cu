@@ -1429,6 +1429,7 @@ kd_attn_status rms_norm_fp8_core(kd_attn_ctx* ctx, const kd_tensor* x, const kd_
     p.gain_align = ga % 32 == 0 ? 32 : (ga % 16 == 0 ? 16 : 1);
     if (gain && p.gain_align < 16) p.align = 1;  // one layout of columns over the lanes for all operands
     p.eps = eps;
+    p.inv_cols = 1.0f / (float)p.out.K;
     KD_CUDA(ctx, launch_norm8(x->type, p, ctx->num_sms, st));
     return KD_ATTN_OK;
 }

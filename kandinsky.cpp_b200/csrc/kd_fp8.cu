@@ -9,6 +9,7 @@
 // A warp's unit of work is 512 columns of a row: four blocks, one 32-bit word of scale bytes, sixteen columns a lane.
 // Where rows start on 16-byte boundaries a lane holds sixteen consecutive columns and moves them in wide accesses;
 // elsewhere (odd row lengths) lane l holds columns l, l + 32, ..., so that its narrow accesses are still coalesced.
+#include <algorithm>
 #include <type_traits>
 
 #include "kd_fp8.cuh"
@@ -77,6 +78,51 @@ __device__ __forceinline__ void put(Raw<T>& a, int j, T v) {
     }
 }
 
+// The same two at a time.  These kernels issue an instruction in three cycles of four and more when written value by
+// value, so the arithmetic is packed: pairs of f32 in one instruction, sums of 16-bit rows in their own type (an
+// exact sum rounded once).
+template <typename T>
+__device__ __forceinline__ void add_rows(Raw<T>& x, const Raw<T>& r) {
+#pragma unroll
+    for (int i = 0; i < Raw<T>::kWords; i += 2) {
+        if constexpr (sizeof(T) == 4) {
+            float lo, hi;
+            f2_unpack(add_f32x2(f2_pack(__uint_as_float(x.w[i]), __uint_as_float(x.w[i + 1])),
+                                f2_pack(__uint_as_float(r.w[i]), __uint_as_float(r.w[i + 1]))), lo, hi);
+            x.w[i] = __float_as_uint(lo);
+            x.w[i + 1] = __float_as_uint(hi);
+        } else {
+            using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+#pragma unroll
+            for (int k = i; k < i + 2; ++k) {
+                const T2 s = __hadd2(*reinterpret_cast<const T2*>(&x.w[k]), *reinterpret_cast<const T2*>(&r.w[k]));
+                x.w[k] = *reinterpret_cast<const uint32_t*>(&s);
+            }
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ void widen(const Raw<T>& a, float (&v)[kPer]) {
+#pragma unroll
+    for (int i = 0; i < Raw<T>::kWords; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            v[i] = __uint_as_float(a.w[i]);
+        } else if constexpr (std::is_same<T, __half>::value) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a.w[i]));
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        } else {
+            v[2 * i] = __uint_as_float(a.w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(a.w[i] & 0xFFFF0000u);
+        }
+    }
+}
+__device__ __forceinline__ void scale16(float (&v)[kPer], float s) {
+    const uint64_t ss = f2_pack(s, s);
+#pragma unroll
+    for (int j = 0; j < kPer; j += 2) f2_unpack(mul_f32x2(f2_pack(v[j], v[j + 1]), ss), v[j], v[j + 1]);
+}
+
 // The column of value j of a lane in the chunk from c0.
 template <bool kVec>
 __device__ __forceinline__ int column(int c0, int lane, int j) {
@@ -128,30 +174,30 @@ __device__ __forceinline__ void store16(T* row, int c0, int lane, int K, int ali
 }
 
 // The largest finite magnitude (as bits) of the block of each of a lane's values: kVec: one block a lane, in top[0];
-// else block i holds values 4 i .. 4 i + 3 of every lane.  NaNs and infinities become NaN in v.
+// else block i holds values 4 i .. 4 i + 3 of every lane.  A maximum passes over NaNs; infinities become NaN in v.
 template <bool kVec>
 __device__ __forceinline__ void block_tops(float (&v)[kPer], uint32_t (&top)[4]) {
     constexpr int kBlocks = kVec ? 1 : 4, kIn = kPer / kBlocks;
-    bool odd = false;
+    uint32_t most = 0;
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
-        uint32_t t = 0;
+        float t = fmaxf(fabsf(v[b * kIn]), fabsf(v[b * kIn + 1]));
 #pragma unroll
-        for (int i = 0; i < kIn; ++i) t = max(t, __float_as_uint(fabsf(v[b * kIn + i])));
-        odd |= t >= kInfBits;
-        top[b] = t;
+        for (int i = 2; i < kIn; i += 2) t = fmax3(t, fabsf(v[b * kIn + i]), fabsf(v[b * kIn + i + 1]));
+        t = fmaxf(t, 0.0f);  // all NaN
+        top[b] = __float_as_uint(t);
+        most = max(most, top[b]);
     }
-    if (__any_sync(kAll, odd)) {
+    if (__any_sync(kAll, most >= kInfBits)) {
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) {
-            uint32_t t = 0;
+            float t = 0.0f;
 #pragma unroll
             for (int i = 0; i < kIn; ++i) {
-                const uint32_t a = __float_as_uint(fabsf(v[b * kIn + i]));
-                if (a >= kInfBits) v[b * kIn + i] = __uint_as_float(0x7FFFFFFFu);
-                else t = max(t, a);
+                if (__float_as_uint(fabsf(v[b * kIn + i])) >= kInfBits) v[b * kIn + i] = __uint_as_float(0x7FFFFFFFu);
+                else t = fmaxf(t, fabsf(v[b * kIn + i]));
             }
-            top[b] = t;
+            top[b] = __float_as_uint(t);
         }
     }
 #pragma unroll
@@ -176,14 +222,12 @@ __device__ __forceinline__ void encode16(float (&v)[kPer], const Fp8Rows& o, lon
     if constexpr (kVec) {
         const uint32_t byte = fp8_scale_byte(top[0]);
         word = __reduce_or_sync(kAll, byte << (8 * (lane >> 3)));
-        const float inv = fp8_scale_inverse(byte);  // a power of two: the products are exact
+        scale16(v, fp8_scale_inverse(byte));  // by a power of two: exact
         const int c = column<kVec>(c0, lane, 0);
         if (c < o.K)  // rows are K rounded up to 16 bytes long at least
             *reinterpret_cast<uint4*>(codes + c) =
-                make_uint4(fp8_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
-                           fp8_pack4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv),
-                           fp8_pack4(v[8] * inv, v[9] * inv, v[10] * inv, v[11] * inv),
-                           fp8_pack4(v[12] * inv, v[13] * inv, v[14] * inv, v[15] * inv));
+                make_uint4(fp8_pack4(v[0], v[1], v[2], v[3]), fp8_pack4(v[4], v[5], v[6], v[7]),
+                           fp8_pack4(v[8], v[9], v[10], v[11]), fp8_pack4(v[12], v[13], v[14], v[15]));
     } else {
         word = 0;
 #pragma unroll
@@ -218,19 +262,26 @@ __device__ __forceinline__ void unit_at(long long unit, int ktiles, bool narrow,
         chunk = (int)(unit % ktiles);
     }
 }
-// The start of token row m, L tokens to a sequence (all of them when rows are evenly spaced).
+// The start of token row m, L tokens to a sequence unless rows are evenly spaced.
 template <typename P>
-__device__ __forceinline__ P* row_at(P* base, long long m, long long L, long long rows, long long nb1, long long nb2) {
+__device__ __forceinline__ P* row_at(P* base, long long m, bool even, long long L, long long nb1, long long nb2) {
     using Bytes = typename std::conditional<std::is_const<P>::value, const char, char>::type;
     Bytes* b = reinterpret_cast<Bytes*>(base);
-    return reinterpret_cast<P*>(L >= rows ? b + m * nb1 : b + (m / L) * nb2 + (m % L) * nb1);
+    return reinterpret_cast<P*>(even ? b + m * nb1 : b + (m / L) * nb2 + (m % L) * nb1);
 }
 
-// One row at a time by blockDim.x threads (kWarpRows: by each warp of its own), thread t holding kChunks chunks of 512
-// columns from its warp's place on.  The CTA stays and takes every gridDim.x-th row: the gain is read once, and
+// Threads of the norm that an SM is to hold: 768 (80 registers) for 16-bit rows, whose loads in flight are small, 512
+// (128 registers) for f32.  Measured at 31,744 x 4,096 bf16 with residual: 512 threads 176 us, 768 154 us, 1,024 170 us
+// (spills).
+template <typename T>
+constexpr int norm_threads() { return sizeof(T) == 2 ? 768 : 512; }
+
+// One row at a time by the CTA (kWarpRows: by each warp of its own), a warp holding one chunk of 512 columns, or two
+// in CTAs of more than 512 threads.  The CTA stays and takes every gridDim.x-th row: the gain is read once, and
 // the next row is on its way (in registers) while this one is summed, divided and written.  One pass over the data.
-template <typename T, bool kVec, int kChunks, bool kWarpRows>
-__global__ void __launch_bounds__(kWarpRows ? 128 : (kChunks == 1 ? 512 : 1024)) norm8_kernel(const Norm8Params p) {
+template <typename T, bool kVec, int kMaxThreads, bool kWarpRows>
+__global__ void __launch_bounds__(kMaxThreads, std::max(1, norm_threads<T>() / kMaxThreads)) norm8_kernel(const Norm8Params p) {
+    constexpr int kChunks = kMaxThreads > 512 ? 2 : 1;
     constexpr bool kAhead = kChunks == 1;  // a second row of 32 columns a thread does not fit the registers
     __shared__ float part[2][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
@@ -247,9 +298,10 @@ __global__ void __launch_bounds__(kWarpRows ? 128 : (kChunks == 1 ? 512 : 1024))
 #pragma unroll
         for (int j = 0; j < kPer; ++j) g[q][j] = p.gain && kAhead ? __uint_as_float(a.w[j]) : 1.0f;
     }
+    const bool even = p.L >= rows;
     auto fetch = [&](long long m, Raw<T> (&x)[kChunks], Raw<T> (&r)[kChunks]) {
-        const T* px = row_at(static_cast<const T*>(p.x), m, p.L, rows, p.x_nb1, p.x_nb2);
-        const T* pr = row_at(static_cast<const T*>(p.r), m, p.L, rows, p.r_nb1, p.r_nb2);
+        const T* px = row_at(static_cast<const T*>(p.x), m, even, p.L, p.x_nb1, p.x_nb2);
+        const T* pr = row_at(static_cast<const T*>(p.r), m, even, p.L, p.r_nb1, p.r_nb2);
 #pragma unroll
         for (int q = 0; q < kChunks; ++q) {
             load16<T, kVec>(px, c0 + q * kChunk, lane, K, p.align, x[q]);
@@ -262,30 +314,25 @@ __global__ void __launch_bounds__(kWarpRows ? 128 : (kChunks == 1 ? 512 : 1024))
     for (long long m = first; m < rows; m += step, turn ^= 1) {
         if (!kAhead) fetch(m, x, r);
         float v[kChunks][kPer];
-        float sum = 0.0f;
+        uint64_t sums = f2_pack(0.0f, 0.0f);
 #pragma unroll
         for (int q = 0; q < kChunks; ++q) {
-            if (p.r) {
-                // the sum is rounded to the rows' type, as it is stored, and the norm is of the stored value
+            // the sum is rounded to the rows' type, as it is stored, and the norm is of the stored value
+            if (p.r) add_rows(x[q], r[q]);
+            if (p.h)
+                store16<T, kVec>(row_at(static_cast<T*>(p.h), m, even, p.L, p.h_nb1, p.h_nb2), c0 + q * kChunk, lane, K, p.align,
+                                 x[q]);
+            widen(x[q], v[q]);
 #pragma unroll
-                for (int j = 0; j < kPer; j += 2) {  // (a word at a time: two values of 16 bits share one)
-                    const T lo = from_f32<T>(to_f32(get(x[q], j)) + to_f32(get(r[q], j)));
-                    const T hi = from_f32<T>(to_f32(get(x[q], j + 1)) + to_f32(get(r[q], j + 1)));
-                    put(x[q], j, lo);
-                    put(x[q], j + 1, hi);
-                }
-            }
-            if (p.h) {
-                T* ph = row_at(static_cast<T*>(p.h), m, p.L, rows, p.h_nb1, p.h_nb2);
-                store16<T, kVec>(ph, c0 + q * kChunk, lane, K, p.align, x[q]);
-            }
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                v[q][j] = to_f32(get(x[q], j));
-                sum = fmaf(v[q][j], v[q][j], sum);
+            for (int j = 0; j < kPer; j += 2) {
+                const uint64_t a = f2_pack(v[q][j], v[q][j + 1]);
+                sums = fma_f32x2(a, a, sums);
             }
         }
         if (kAhead && m + step < rows) fetch(m + step, x, r);
+        float sum, other;
+        f2_unpack(sums, sum, other);
+        sum += other;
 #pragma unroll
         for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(kAll, sum, s);
         if (!kWarpRows && warps > 1) {
@@ -296,7 +343,7 @@ __global__ void __launch_bounds__(kWarpRows ? 128 : (kChunks == 1 ? 512 : 1024))
 #pragma unroll
             for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(kAll, sum, s);
         }
-        const float inv = __frcp_rn(__fsqrt_rn(__fadd_rn(__fdiv_rn(sum, (float)K), p.eps)));
+        const float inv = rsqrtf(fmaf(sum, p.inv_cols, p.eps));
 #pragma unroll
         for (int q = 0; q < kChunks; ++q) {
             if (!kAhead && p.gain) {
@@ -305,8 +352,10 @@ __global__ void __launch_bounds__(kWarpRows ? 128 : (kChunks == 1 ? 512 : 1024))
 #pragma unroll
                 for (int j = 0; j < kPer; ++j) g[q][j] = __uint_as_float(a.w[j]);
             }
+            scale16(v[q], inv);
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) v[q][j] = v[q][j] * inv * g[q][j];
+            for (int j = 0; j < kPer; j += 2)
+                f2_unpack(mul_f32x2(f2_pack(v[q][j], v[q][j + 1]), f2_pack(g[q][j], g[q][j + 1])), v[q][j], v[q][j + 1]);
             if (c0 + q * kChunk < K) encode16<kVec>(v[q], p.out, m, c0 + q * kChunk, lane);
         }
     }
@@ -324,11 +373,10 @@ __global__ void __launch_bounds__(kUnitThreads) quant8_kernel(const Quant8Params
     int chunk;
     unit_at(unit, p.out.ktiles, units <= 0xffffffffll, row, chunk);
     Raw<T> a;
-    load16<T, kVec>(row_at(static_cast<const T*>(p.x), row, p.L, p.out.rows, p.x_nb1, p.x_nb2), chunk * kChunk, lane, p.out.K,
+    load16<T, kVec>(row_at(static_cast<const T*>(p.x), row, p.L >= p.out.rows, p.L, p.x_nb1, p.x_nb2), chunk * kChunk, lane, p.out.K,
                     p.align, a);
     float v[kPer];
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) v[j] = to_f32(get(a, j));
+    widen(a, v);
     encode16<kVec>(v, p.out, row, chunk * kChunk, lane);
 }
 
@@ -439,25 +487,35 @@ __global__ void __launch_bounds__(kUnitThreads) dequant8_kernel(const Dequant8Pa
             float v[4];
             fp8_unpack4(codes[u][i], v);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) put(a, 4 * i + j, from_f32<T>(v[j] * s));
+            for (int j = 0; j < 4; j += 2) {
+                f2_unpack(mul_f32x2(f2_pack(v[j], v[j + 1]), f2_pack(s, s)), v[j], v[j + 1]);
+                if constexpr (sizeof(T) == 4) {
+                    a.w[4 * i + j] = __float_as_uint(v[j]);
+                    a.w[4 * i + j + 1] = __float_as_uint(v[j + 1]);
+                } else {
+                    a.w[2 * i + (j >> 1)] = Pack2<T>::pack(v[j], v[j + 1]);
+                }
+            }
         }
-        store16<T, kVec>(row_at(static_cast<T*>(p.y), row[u], p.L, p.in.rows, p.y_nb1, p.y_nb2), c0[u], lane, p.in.K, p.align, a);
+        store16<T, kVec>(row_at(static_cast<T*>(p.y), row[u], p.L >= p.in.rows, p.L, p.y_nb1, p.y_nb2), c0[u], lane, p.in.K, p.align, a);
     }
 }
 
-// Up to 512 columns a warp has a row of its own; to 8,192 one CTA of a warp for every 512 columns; above, a warp for
+// Up to 512 columns a warp has a row of its own; to 8,192 a CTA has a warp for every 512 columns; above, a warp for
 // every 1,024.  CTAs stay for as many rows as fill the GPU.
 template <typename T, bool kVec>
 cudaError_t norm8_typed(const Norm8Params& p, int num_sms, cudaStream_t st) {
     const int K = p.out.K;
-    const bool warp_rows = K <= kChunk;
-    const int chunks = K <= 16 * kChunk ? 1 : 2;
-    const int threads = warp_rows ? 128 : (K + chunks * kChunk - 1) / (chunks * kChunk) * 32;
-    auto kern = warp_rows ? norm8_kernel<T, kVec, 1, true>
-                          : (chunks == 1 ? norm8_kernel<T, kVec, 1, false> : norm8_kernel<T, kVec, 2, false>);
-    const long long per_cta = warp_rows ? 4 : 1;
-    const long long want = (p.out.rows + per_cta - 1) / per_cta, fit = (long long)num_sms * (1024 / threads);
-    kern<<<(unsigned)(want < fit ? want : fit), threads, 0, st>>>(p);
+    const int chunk = K <= 16 * kChunk ? kChunk : 2 * kChunk;
+    const int threads = K <= kChunk ? 128 : (K + chunk - 1) / chunk * 32;
+    auto kern = K <= kChunk        ? norm8_kernel<T, kVec, 128, true>
+                : K <= 8 * kChunk  ? norm8_kernel<T, kVec, 256, false>
+                : K <= 16 * kChunk ? norm8_kernel<T, kVec, 512, false>
+                                   : norm8_kernel<T, kVec, 1024, false>;
+    const long long per_cta = K <= kChunk ? 4 : 1;
+    const long long want = (p.out.rows + per_cta - 1) / per_cta;
+    const long long fit = (long long)num_sms * std::max(1, norm_threads<T>() / threads);
+    kern<<<(unsigned)std::min(want, fit), threads, 0, st>>>(p);
     return cudaGetLastError();
 }
 

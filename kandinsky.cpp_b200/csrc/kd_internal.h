@@ -200,7 +200,7 @@ struct Norm8Params {
     long long x_nb1, x_nb2, r_nb1, r_nb2, h_nb1, h_nb2;
     int align, gain_align;             // bytes that every row of x, r and h starts on: 32, 16, or less; gain's address
     long long L;                       // tokens per sequence
-    float eps;
+    float eps, inv_cols;               // inv_cols = 1 / K
     Fp8Rows out;                       // L * N rows
 };
 struct Quant8Params {
