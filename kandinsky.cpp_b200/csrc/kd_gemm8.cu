@@ -7,6 +7,8 @@
 // work outside the tensor core.  The instruction covers 32 columns and selects its scale byte by the descriptor's
 // scale id; the four instructions of a block name the same byte, and one 32-bit TMEM column holds the bytes of four
 // blocks (512 columns).
+#include <atomic>
+
 #include "kd_fp8.cuh"
 #include "kd_internal.h"
 
@@ -88,6 +90,19 @@ template <>
 __device__ __forceinline__ __half round_to<__half>(float v) { return __float2half_rn(v); }
 template <>
 __device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Allows a kernel its dynamic shared memory, once on each device.
+template <typename K>
+cudaError_t allow_smem(K kern, int bytes, std::atomic<unsigned long long>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_release);
+    return e;
+}
 
 // The output row of token m; L tokens to a sequence (all of them when the rows are evenly spaced).
 __device__ __forceinline__ char* token_row(const Gemm8Params& p, int m) {
@@ -674,7 +689,8 @@ __global__ void __launch_bounds__(kPThreads, 1)
 template <typename TO, int kParts>
 cudaError_t many_typed(const CUtensorMap* tm, const Gemm8Params& p, int num_sms, cudaStream_t st) {
     auto kern = gemm8_many_kernel<TO, kParts>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPSmem);
+    static std::atomic<unsigned long long> ready{0};
+    cudaError_t e = allow_smem(kern, kPSmem, ready);
     if (e != cudaSuccess) return e;
     const long long tiles = (long long)((p.M + kPairM - 1) / kPairM) * ((p.N + p.nt * p.parts - 1) / (p.nt * p.parts));
     cudaLaunchConfig_t cfg{};
@@ -701,7 +717,8 @@ cudaError_t many_typed(const CUtensorMap* tm, const Gemm8Params& p, int num_sms,
 template <typename TO>
 cudaError_t few_typed(const CUtensorMap& tmX, const CUtensorMap& tmW, const Gemm8Params& p, cudaStream_t st) {
     auto kern = gemm8_few_kernel<TO>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSSmem);
+    static std::atomic<unsigned long long> ready{0};
+    cudaError_t e = allow_smem(kern, kSSmem, ready);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[1];
