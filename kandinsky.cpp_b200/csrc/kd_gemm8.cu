@@ -7,6 +7,7 @@
 // work outside the tensor core.  The instruction covers 32 columns and selects its scale byte by the descriptor's
 // scale id; the four instructions of a block name the same byte, and one 32-bit TMEM column holds the bytes of four
 // blocks (512 columns).
+#include <algorithm>
 #include <atomic>
 
 #include "kd_fp8.cuh"
@@ -16,18 +17,32 @@ namespace kd {
 namespace {
 
 // ------------------------------------------------------------------ primitives
-// D[tmem] (+)= A * B with block scales at sa / sb in TMEM; executed by a converged warp, issued by one lane.
-__device__ __forceinline__ void mma8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                        uint32_t sa, uint32_t sb, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred e, p;\n\t"
-        "elect.sync _|e, 0xffffffff;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(
-            d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
-        : "memory");
+// The four MMAs of a block of 128 columns, D[tmem] (+)= A * B with block scales at sa / sb in TMEM, their operands 32
+// bytes of each row apart; executed by a converged warp, issued by one lane.  One warp issues all MMAs of a tile, so
+// its instructions count: with an election and descriptors for each MMA, and the ring's and the parts' bookkeeping at
+// run time, the loop of the pair kernel took 1,700 cycles a block where its MMAs take 768.
+#define KD_MMA8_BLOCK(group)                                                                                              \
+    "{\n\t.reg .pred e, p, t;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"                                                   \
+    "elect.sync _|e, 0xffffffff;\n\t"                                                                                     \
+    "setp.ne.b32 p, %6, 0;\n\t"                                                                                           \
+    "setp.eq.b32 t, 0, 0;\n\t"                                                                                            \
+    "add.s64 a1, %1, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 a3, %1, 6;\n\t"                                                  \
+    "add.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"                                                  \
+    "@e tcgen05.mma.cta_group::" group ".kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t"   \
+    "@e tcgen05.mma.cta_group::" group ".kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a1, b1, %3, [%4], [%5], t;\n\t"   \
+    "@e tcgen05.mma.cta_group::" group ".kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a2, b2, %3, [%4], [%5], t;\n\t"   \
+    "@e tcgen05.mma.cta_group::" group ".kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a3, b3, %3, [%4], [%5], t;\n\t}\n"
+template <int kGroup>
+__device__ __forceinline__ void mma8_block(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sa,
+                                           uint32_t sb, uint32_t accumulate) {
+    if constexpr (kGroup == 1)
+        asm volatile(KD_MMA8_BLOCK("1")::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+                     : "memory");
+    else
+        asm volatile(KD_MMA8_BLOCK("2")::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+                     : "memory");
 }
+#undef KD_MMA8_BLOCK
 // One 512-byte scale tile from shared memory into four TMEM columns (32 lanes, repeated for the four lane groups).
 // tcgen05.cp and tcgen05.mma of one thread execute in the order of issue.
 __device__ __forceinline__ void scales_to_tmem(uint32_t tmem, uint64_t desc) {
@@ -114,59 +129,94 @@ __device__ __forceinline__ char* token_row(const Gemm8Params& p, int m) {
 // ------------------------------------------------------------------ few tokens
 // One CTA: 128 output features (the MMA's M) x nt tokens (its N) over a range of K blocks.  With few tokens the
 // weight's bytes are the work, so weights are the operand of full height and the tokens only widen the instruction.
-// The K range is split over a cluster when the feature tiles alone do not fill the GPU; the parts are joined
+// The K range is split over a cluster when that spreads the bytes better over the SMs; the parts are joined
 // through distributed shared memory in the order of the ranks, so results do not depend on timing.
-// A stage is one block of 128 columns: 16 KB of weights, nt * 128 bytes of tokens, and both scale tiles.
-constexpr int kSStages = 4;
+// A stage is one block of 128 columns: 16 KB of weights, nt * 128 bytes of tokens, and both scale tiles.  Shared memory
+// and TMEM are taken as needed, so that CTAs with few blocks share an SM and one's copies run under another's join.
 constexpr int kSWeightBytes = kGemm8BoxRows * 128;
-constexpr int kSTokenBytes = kGemm8MaxTokens * 128;
-constexpr int kSScaleBytes = 3 * 512;                       // weights' tile, up to two tiles of tokens
-constexpr int kSStageBytes = kSWeightBytes + kSTokenBytes;  // 48 KB
-constexpr int kSScaleAt = kSStages * kSStageBytes;
-constexpr int kSBarAt = kSScaleAt + kSStages * kSScaleBytes;
-constexpr int kSNumBars = 2 * kSStages + 1;                 // full, empty, accumulator complete
-constexpr int kSSlotAt = kSBarAt + kSNumBars * 8;           // TMEM address, abort flag
-constexpr int kSSmem = kSSlotAt + 16 + 1024;
-static_assert(kSSmem <= 232448, "shared memory budget");
-static_assert(kGemm8MaxTokens * 128 * 4 <= kSScaleAt, "the partial sums reuse the stages");
-constexpr int kSThreads = 192;  // warp 0 copies, warp 1 issues MMAs, warps 2-5 read the accumulator
-constexpr uint32_t kSTmemCols = 512;
-constexpr uint32_t kSScaleCol = 256;  // two sets of scale columns: 4 of the weights, 8 of the tokens
+constexpr int kSScaleBytes = 3 * 512;  // weights' tile, up to two tiles of tokens
+constexpr int kSMaxStages = 12;
+constexpr int kSFixed = (2 * kSMaxStages + 1) * 8 + 16 + 1024;  // barriers, TMEM address and abort flag, alignment
+constexpr int kSJoinWarps = 8, kSThreads = 32 * (2 + kSJoinWarps);  // warp 0 copies, warp 1 issues MMAs, the others join
+constexpr uint32_t kSScaleCols = 32;  // two sets of scale columns: 4 of the weights, 8 of the tokens
+
+__host__ __device__ constexpr int few_stage_bytes(int nt) { return kSWeightBytes + nt * 128; }
+// Stages of a CTA with nk blocks: all of them if they fit (with their scales) and room for the sums at least.
+__host__ __device__ constexpr int few_stages(int nt, int nk) {
+    const int fit = (232448 - kSFixed) / (few_stage_bytes(nt) + kSScaleBytes);
+    const int most = fit < kSMaxStages ? fit : kSMaxStages;
+    const int sums = (nt * 512 + few_stage_bytes(nt) - 1) / few_stage_bytes(nt);
+    const int want = nk > sums ? nk : sums;
+    return want < most ? want : most;
+}
+static_assert(few_stages(kGemm8MaxTokens, 1) * few_stage_bytes(kGemm8MaxTokens) >= kGemm8MaxTokens * 512, "room for the sums");
+__host__ __device__ constexpr uint32_t few_tmem_cols(int nt) {
+    return nt + kSScaleCols <= 64 ? 64 : (nt + kSScaleCols <= 128 ? 128 : (nt + kSScaleCols <= 256 ? 256 : 512));
+}
+// At least the share of the SM's 228 KB (1 KB a CTA is the system's) that the CTA takes of its 512 TMEM columns: CTAs that
+// share an SM then never wait for each other's columns, which clusters that wait for their own CTAs could do for good.
+constexpr int few_smem(int nt, int nk) {
+    const int need = few_stages(nt, nk) * (few_stage_bytes(nt) + kSScaleBytes) + kSFixed;
+    const int share = (int)few_tmem_cols(nt) * (233472 / 512) - 1024;
+    return need > share ? need : share;
+}
 
 template <typename TO>
-__global__ void __launch_bounds__(kSThreads, 1)
+__global__ void __launch_bounds__(kSThreads)
     gemm8_few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                      const __grid_constant__ Gemm8Params p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t base = smem_u32(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + kSBarAt);
-    uint64_t* empty = full + kSStages;
-    uint64_t* done = empty + kSStages;
-    uint32_t* slot = reinterpret_cast<uint32_t*>(smem + kSSlotAt);
-    unsigned* abort_flag = slot + 1;  // of this CTA alone
-    const DevCtl ctl{p.err, abort_flag, p.wait_ns};
 
     const uint32_t rank = cluster_rank();
     const int n0 = (int)(blockIdx.x / p.splits) * kGemm8BoxRows;
-    const int m0 = (int)blockIdx.y * p.nt;
     const int blocks = (p.K + 127) >> 7;
     const int k0 = (int)((long long)blocks * rank / p.splits), k1 = (int)((long long)blocks * (rank + 1) / p.splits);
     const int nk = k1 - k0;  // at least 1: splits <= blocks
-    const int token_tiles = (min(p.M - m0, p.nt) + 127) >> 7;
+    const int token_tiles = (p.M + 127) >> 7;
+    const bool direct = p.splits == 1 && p.nt == 16;  // sums of few tokens are stored from where they are
+    // the ring's size goes by the largest part, as the host's
+    const int stages = few_stages(p.nt, (blocks + p.splits - 1) / p.splits);
+    const uint32_t stage_bytes = few_stage_bytes(p.nt), scale_at = stages * stage_bytes;
+    const uint32_t cols = few_tmem_cols(p.nt), scale_col = cols - kSScaleCols;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + scale_at + stages * kSScaleBytes);
+    uint64_t* empty = full + kSMaxStages;
+    uint64_t* done = empty + kSMaxStages;
+    uint32_t* slot = reinterpret_cast<uint32_t*>(done + 1);
+    unsigned* abort_flag = slot + 1;  // of this CTA alone
+    const DevCtl ctl{p.err, abort_flag, p.wait_ns};
 
+    auto copy_block = [&](int i, int s) {  // block i of this CTA into stage s
+        const uint32_t bar = smem_u32(&full[s]), st = base + s * stage_bytes, sc = base + scale_at + s * kSScaleBytes;
+        const int kb = k0 + i;
+        const bool scales = i == 0 || (kb & 3) == 0;  // a scale tile covers four blocks
+        mbar_arrive_expect_tx(&full[s], stage_bytes + (scales ? 512u * (1 + token_tiles) : 0u));
+        tma_load_2d(st, &tmW, bar, kb * 128, n0);
+        tma_load_2d(st + kSWeightBytes, &tmX, bar, kb * 128, 0);
+        if (scales) {
+            bulk_load(sc, p.w_scales + fp8_scale_offset(n0, kb & ~3, p.ktiles), 512, bar);
+            for (int t = 0; t < token_tiles; ++t)
+                bulk_load(sc + 512 * (1 + t), p.x_scales + fp8_scale_offset(128 * t, kb & ~3, p.ktiles), 512, bar);
+        }
+    };
+
+    // The first stages are on their way before the CTA meets: their copies need nothing but the barriers.
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kSStages; ++s) {
+        tma_prefetch_desc(&tmW);
+        tma_prefetch_desc(&tmX);
+        for (int s = 0; s < stages; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
         mbar_init(done, 1);
         *abort_flag = 0;
         fence_mbar_init();
+        for (int i = 0; i < min(nk, stages); ++i) copy_block(i, i);
     }
     if (warp == 1) {
-        tmem_alloc(slot, kSTmemCols);
+        tmem_alloc(slot, cols);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -175,47 +225,34 @@ __global__ void __launch_bounds__(kSThreads, 1)
     const uint32_t tmem = *slot;
 
     if (warp == 0) {
-        const uint32_t bytes = kSWeightBytes + (uint32_t)p.nt * 128u + 512u * (1 + token_tiles);
-        bool ok = true;
-        for (int i = 0; i < nk; ++i) {
-            const int s = i % kSStages;
-            if (!(ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((i / kSStages) & 1u) ^ 1u, ctl, kErrTimeoutKVEmpty))))
-                break;
-            if (lane == 0) {
-                const uint32_t bar = smem_u32(&full[s]), st = base + s * kSStageBytes;
-                const uint32_t sc = base + kSScaleAt + s * kSScaleBytes;
-                const int kb = k0 + i;
-                mbar_arrive_expect_tx(&full[s], bytes);
-                tma_load_2d(st, &tmW, bar, kb * 128, n0);
-                tma_load_2d(st + kSWeightBytes, &tmX, bar, kb * 128, m0);
-                bulk_load(sc, p.w_scales + fp8_scale_offset(n0, kb & ~3, p.ktiles), 512, bar);
-                for (int t = 0; t < token_tiles; ++t)
-                    bulk_load(sc + 512 * (1 + t), p.x_scales + fp8_scale_offset(m0 + 128 * t, kb & ~3, p.ktiles), 512, bar);
-            }
+        for (int i = stages; i < nk; ++i) {
+            const int s = i % stages;
+            if (!__all_sync(0xffffffffu, mbar_wait(&empty[s], ((i / stages) & 1u) ^ 1u, ctl, kErrTimeoutKVEmpty))) break;
+            if (lane == 0) copy_block(i, s);
             __syncwarp();
         }
     } else if (warp == 1) {
         constexpr uint32_t dhi = sw128_desc_hi(1024);
+        const uint32_t idesc0 = idesc_e4m3_block(128, p.nt, 0);
+        uint32_t sa = tmem + scale_col;  // the two sets differ in bit 4
         bool ok = true;
-        int i = 0;
+        int i = 0, s = 0, turn = 0;
         for (; i < nk; ++i) {
-            const int s = i % kSStages, kb = k0 + i;
-            if (!(ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (i / kSStages) & 1u, ctl, kErrTimeoutKVFull)))) break;
+            const int kb = k0 + i;
+            if (!(ok = __all_sync(0xffffffffu, mbar_wait(&full[s], turn & 1u, ctl, kErrTimeoutKVFull)))) break;
             tc_fence_after();
-            const uint32_t sa = tmem + kSScaleCol + 16u * (uint32_t)((kb >> 2) & 1), sb = sa + 4;
-            if (i == 0 || (kb & 3) == 0) {  // four blocks share a tile
-                const uint32_t sc = base + kSScaleAt + s * kSScaleBytes;
+            if (i == 0 || (kb & 3) == 0) {
+                sa ^= 16u;
+                const uint32_t sc = base + scale_at + s * kSScaleBytes;
                 scales_to_tmem(sa, desc_scale_tile(sc));
-                for (int t = 0; t < token_tiles; ++t) scales_to_tmem(sb + 4 * t, desc_scale_tile(sc + 512 * (1 + t)));
+                for (int t = 0; t < token_tiles; ++t) scales_to_tmem(sa + 4 + 4 * t, desc_scale_tile(sc + 512 * (1 + t)));
             }
-            const uint32_t idesc = idesc_e4m3_block(128, p.nt, kb & 3);
-            const uint32_t alo = sw128_desc_lo(base + s * kSStageBytes, 16);
-            const uint32_t blo = sw128_desc_lo(base + s * kSStageBytes + kSWeightBytes, 16);
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-                mma8_ss(tmem, desc_join(alo + kk * 2, dhi), desc_join(blo + kk * 2, dhi), idesc, sa, sb,
-                        (i | kk) ? 1u : 0u);
+            const uint32_t idesc = idesc0 | ((uint32_t)(kb & 3) << 4) | ((uint32_t)(kb & 3) << 29);
+            const uint32_t alo = sw128_desc_lo(base + s * stage_bytes, 16);
+            const uint32_t blo = sw128_desc_lo(base + s * stage_bytes + kSWeightBytes, 16);
+            mma8_block<1>(tmem, desc_join(alo, dhi), desc_join(blo, dhi), idesc, sa, sa + 4, i ? 1u : 0u);
             tc_commit(&empty[s]);
+            if (++s == stages) s = 0, ++turn;
         }
         if (ok) {
             tc_commit(done);
@@ -224,30 +261,24 @@ __global__ void __launch_bounds__(kSThreads, 1)
             mbar_wait(done, 0, ctl, kErrTimeoutDrain, false);
         }
     } else {
-        const int q = warp & 3;  // TMEM lanes 32 q .. of this warp
+        const int q = warp & 3, half = (warp - 2) >> 2;  // TMEM lanes 32 q .. of this warp, every other 16 columns
         const int f = q * 32 + lane, n = n0 + f;
+        const float bias = direct && p.bias && n < p.N ? __ldg(p.bias + n) : 0.0f;
         const bool ok = __all_sync(0xffffffffu, mbar_wait(done, 0, ctl, kErrTimeoutO));
         tc_fence_after();
         if (ok && *reinterpret_cast<volatile unsigned*>(abort_flag) == 0) {
             const uint32_t src = tmem + ((uint32_t)(q * 32) << 16);
-            if (p.splits == 1) {
-                const float bias = p.bias && n < p.N ? __ldg(p.bias + n) : 0.0f;
-                for (int c = 0; c < p.nt; c += 16) {
-                    float v[16];
-                    tmem_ld16_sync(src + c, v);
+            // all copies have been consumed by completed MMAs: the stages may hold the sums [token][feature] now
+            float* part = reinterpret_cast<float*>(smem);
+            for (int c = half * 16; c < p.nt; c += 32) {
+                float v[16];
+                tmem_ld16_sync(src + c, v);
+                if (direct) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const int m = m0 + c + j;
-                        if (m < p.M && n < p.N)
-                            reinterpret_cast<TO*>(token_row(p, m))[n] = round_to<TO>(v[j] + bias);
-                    }
-                }
-            } else {
-                // all copies have been consumed by completed MMAs: the stages hold the sums [token][feature] now
-                float* part = reinterpret_cast<float*>(smem);
-                for (int c = 0; c < p.nt; c += 16) {
-                    float v[16];
-                    tmem_ld16_sync(src + c, v);
+                    for (int j = 0; j < 16; ++j)
+                        if (c + j < p.M && n < p.N)
+                            reinterpret_cast<TO*>(token_row(p, c + j))[n] = round_to<TO>(v[j] + bias);
+                } else {
 #pragma unroll
                     for (int j = 0; j < 16; ++j) part[(c + j) * 128 + f] = v[j];
                 }
@@ -255,27 +286,51 @@ __global__ void __launch_bounds__(kSThreads, 1)
         }
         tc_fence_before();
     }
-    if (p.splits > 1) {
+    if (!direct) {
         __syncwarp();
         cluster_sync_all();  // every rank's sums are in its shared memory
         if (warp >= 2) {
-            const int tokens = min(p.M - m0, p.nt);
-            const int n = n0 + lane * 4;
+            // A warp adds the ranks' sums of 128 features, two tokens at a time: their reads, from the other SMs, are
+            // under way together.
+            const int n = n0 + lane * 4, step = p.splits * kSJoinWarps;
             float b[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) b[j] = p.bias && n + j < p.N ? __ldg(p.bias + n + j) : 0.0f;
-            for (int c = (int)rank + p.splits * (warp - 2); c < tokens; c += 4 * p.splits) {
-                float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (int r = 0; r < p.splits; ++r) {
-                    const float4 v = ld_cluster_v4(base + (uint32_t)(c * 128 + lane * 4) * 4u, (uint32_t)r);
-                    a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
-                }
-                const int m = m0 + c;
-                TO* y = reinterpret_cast<TO*>(token_row(p, m)) + n;
-                const float v[4] = {a.x + b[0], a.y + b[1], a.z + b[2], a.w + b[3]};
+            for (int c0 = (int)rank + p.splits * (warp - 2); c0 < p.M; c0 += 2 * step) {
+                float4 a[2];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (n + j < p.N) y[j] = round_to<TO>(v[j]);
+                for (int r0 = 0; r0 < 8; r0 += 4) {
+                    if (r0 >= p.splits) break;
+                    float4 v[2][4];
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (r0 + r < p.splits && c0 + t * step < p.M)
+                                v[t][r] = ld_cluster_v4(base + (uint32_t)((c0 + t * step) * 128 + lane * 4) * 4u, (uint32_t)(r0 + r));
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        if (r0 == 0) a[t] = v[t][0];
+#pragma unroll
+                        for (int r = r0 == 0 ? 1 : 0; r < 4; ++r)
+                            if (r0 + r < p.splits) a[t].x += v[t][r].x, a[t].y += v[t][r].y, a[t].z += v[t][r].z, a[t].w += v[t][r].w;
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int c = c0 + t * step;
+                    if (c >= p.M) break;
+                    TO* y = reinterpret_cast<TO*>(token_row(p, c)) + n;
+                    const float w[4] = {a[t].x + b[0], a[t].y + b[1], a[t].z + b[2], a[t].w + b[3]};
+                    if (p.y_vec && n + 4 <= p.N) {  // (32-byte aligned rows: four values are 8 or 16 aligned bytes)
+                        if constexpr (sizeof(TO) == 4) *reinterpret_cast<float4*>(y) = make_float4(w[0], w[1], w[2], w[3]);
+                        else *reinterpret_cast<uint2*>(y) = make_uint2(Pack2<TO>::pack(w[0], w[1]), Pack2<TO>::pack(w[2], w[3]));
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (n + j < p.N) y[j] = round_to<TO>(w[j]);
+                    }
+                }
             }
         }
         __syncwarp();
@@ -291,7 +346,7 @@ __global__ void __launch_bounds__(kSThreads, 1)
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, kSTmemCols);
+        tmem_dealloc(tmem, cols);
     }
 }
 
@@ -321,7 +376,7 @@ constexpr int kPSmem = kPSlotAt + 16 + 1024;
 static_assert(kPSmem <= 232448, "shared memory budget");
 // Two groups of eight epilogue warps, one for each accumulator, then the copy warp and the MMA warp.
 constexpr int kPGroupWarps = 8, kPEpiWarps = 16, kPThreads = 32 * (kPEpiWarps + 2);
-constexpr uint32_t kPAccCols = 192;
+constexpr uint32_t kPTmemCols = 512, kPAccCols = 192;
 constexpr uint32_t kPScaleCol = 384;  // two sets: 4 columns of the tokens, 12 of the features
 constexpr int kBandM = 8;  // token tiles swept together, so that the tiles in flight share operands in L2
 
@@ -346,26 +401,6 @@ __device__ __forceinline__ void tma_pair_3d(uint32_t dst, const CUtensorMap* map
         "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
         " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
-        : "memory");
-}
-// The four MMAs of a block of 128 columns (32 bytes of each operand row apart), issued by one lane.  One warp issues
-// all MMAs of a pair, so its instructions count: with an election and a descriptor for each MMA, and the ring's and
-// the parts' bookkeeping at run time, the loop took 1,700 cycles a block where the MMAs take 768.
-__device__ __forceinline__ void mma8_pair_block(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                                uint32_t sa, uint32_t sb, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred e, p, t;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
-        "elect.sync _|e, 0xffffffff;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "setp.eq.b32 t, 0, 0;\n\t"
-        "add.s64 a1, %1, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 a3, %1, 6;\n\t"
-        "add.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"
-        "@e tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
-        "@e tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a1, b1, %3, [%4], [%5], t;\n\t"
-        "@e tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a2, b2, %3, [%4], [%5], t;\n\t"
-        "@e tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a3, b3, %3, [%4], [%5], t;\n\t}\n" ::"r"(
-            d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
         : "memory");
 }
 // The scale tile at the same offset in both CTAs' shared memory into the same columns of both CTAs' TMEM.
@@ -456,7 +491,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
         fence_mbar_init();
     }
     if (warp == kPEpiWarps + 1) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(kSTmemCols)
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(kPTmemCols)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
@@ -541,7 +576,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
                 if (++s == stages) s = 0, ++turn, lo = lo0;
             };
             auto part = [&](int i, int h, uint32_t acc, uint32_t stage_lo, uint32_t set, uint32_t col) {
-                mma8_pair_block(tmem + acc * kPAccCols, desc_join(stage_lo, dhi),
+                mma8_block<2>(tmem + acc * kPAccCols, desc_join(stage_lo, dhi),
                                 desc_join(stage_lo + (kPTokenBytes >> 4) + h * part_lo, dhi), idesc0 + (uint32_t)(i & 3) * kNextId,
                                 set, set + 4 + col + h * part_col, i ? 1u : 0u);
             };
@@ -682,7 +717,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
     cluster_sync_all();  // no CTA leaves while its partner may still signal its barriers
     if (warp == kPEpiWarps + 1) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kSTmemCols) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kPTmemCols) : "memory");
     }
 }
 
@@ -718,17 +753,16 @@ template <typename TO>
 cudaError_t few_typed(const CUtensorMap& tmX, const CUtensorMap& tmW, const Gemm8Params& p, cudaStream_t st) {
     auto kern = gemm8_few_kernel<TO>;
     static std::atomic<unsigned long long> ready{0};
-    cudaError_t e = allow_smem(kern, kSSmem, ready);
+    cudaError_t e = allow_smem(kern, 232448, ready);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = (unsigned)p.splits;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned)((p.N + kGemm8BoxRows - 1) / kGemm8BoxRows) * (unsigned)p.splits,
-                       (unsigned)((p.M + p.nt - 1) / p.nt));
+    cfg.gridDim = dim3((unsigned)((p.N + kGemm8BoxRows - 1) / kGemm8BoxRows) * (unsigned)p.splits);
     cfg.blockDim = dim3(kSThreads);
-    cfg.dynamicSmemBytes = kSSmem;
+    cfg.dynamicSmemBytes = few_smem(p.nt, ((p.K + 127) / 128 + p.splits - 1) / p.splits);
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
@@ -737,8 +771,9 @@ cudaError_t few_typed(const CUtensorMap& tmX, const CUtensorMap& tmW, const Gemm
 
 }  // namespace
 
-// Few tokens (at most 256): all of them in one tile, in steps of 16; K is split while the tiles leave more than half
-// of the SMs idle and each part keeps at least two blocks, over at most 8 CTAs (the portable cluster size).
+// Few tokens (at most 256): all of them in one tile, in steps of 16; K split over up to 8 CTAs (the portable cluster
+// size) as far as all CTAs run at one time.  (More and shorter CTAs, 3 to 7 to an SM, were slower: 16,384 x 4,096 x
+// one token 14.5 us unsplit, 19.3 us in two parts, 26 us in four.)
 // Many tokens: the tile whose rounds over the SM pairs take the fewest cycles, by the cost of a block of 128 columns
 // (MMAs for two parts of 192, copies for one of 192 or 128, as measured above) and about 1,000 cycles a tile.
 void gemm8_plan(Gemm8Params* p, int num_sms) {
@@ -748,7 +783,7 @@ void gemm8_plan(Gemm8Params* p, int num_sms) {
     if (!p->many) {
         p->nt = (p->M + 15) / 16 * 16;
         const long long tiles = (p->N + kGemm8BoxRows - 1) / kGemm8BoxRows;
-        while (p->splits < 8 && tiles * p->splits * 2 <= num_sms && blocks >= p->splits * 4) p->splits *= 2;
+        p->splits = (int)std::min<long long>(std::min(8, blocks), std::max<long long>(1, num_sms / tiles));
         return;
     }
     const struct { int parts, pn, block_cycles; } shapes[] = {{2, 192, 768}, {1, 192, 494}, {1, 128, 424}};
