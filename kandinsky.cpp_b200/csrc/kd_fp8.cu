@@ -286,6 +286,8 @@ __global__ void __launch_bounds__(kMaxThreads, std::max(1, norm_threads<T>() / k
     __shared__ float part[2][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int K = p.out.K;
+    launch_next();
+    wait_for_previous();
     const int c0 = kWarpRows ? 0 : warp * (kChunks * kChunk);
     const long long first = kWarpRows ? (long long)blockIdx.x * warps + warp : blockIdx.x;
     const long long step = kWarpRows ? (long long)gridDim.x * warps : gridDim.x;
@@ -368,6 +370,8 @@ __global__ void __launch_bounds__(kUnitThreads) quant8_kernel(const Quant8Params
     const int lane = threadIdx.x & 31;
     const long long unit = (long long)blockIdx.x * (kUnitThreads / 32) + (threadIdx.x >> 5);
     const long long units = p.out.rows * p.out.ktiles;
+    launch_next();
+    wait_for_previous();
     if (unit >= units) return;
     long long row;
     int chunk;
@@ -386,6 +390,8 @@ __global__ void __launch_bounds__(kUnitThreads) quant8_kernel(const Quant8Params
 __global__ void quant8_ggml_kernel(const uint8_t* w, int q4, long long row_bytes, const Fp8Rows o) {
     const int blocks = (o.K + 127) >> 7;
     const long long total = o.rows * blocks;
+    launch_next();
+    wait_for_previous();
     const long long step = ((long long)gridDim.x * blockDim.x) >> 2;
     for (long long i = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 2; (i & ~7ll) < total; i += step) {
         const bool live = i < total;
@@ -450,6 +456,8 @@ __global__ void __launch_bounds__(kUnitThreads) dequant8_kernel(const Dequant8Pa
     const int lane = threadIdx.x & 31;
     const long long units = p.in.rows * p.in.ktiles;
     const bool narrow = units <= 0xffffffffll;
+    launch_next();
+    wait_for_previous();
     long long row[kUnits];
     int c0[kUnits];
     uint32_t codes[kUnits][4], word[kUnits];
@@ -515,8 +523,7 @@ cudaError_t norm8_typed(const Norm8Params& p, int num_sms, cudaStream_t st) {
     const long long per_cta = K <= kChunk ? 4 : 1;
     const long long want = (p.out.rows + per_cta - 1) / per_cta;
     const long long fit = (long long)num_sms * std::max(1, norm_threads<T>() / threads);
-    kern<<<(unsigned)std::min(want, fit), threads, 0, st>>>(p);
-    return cudaGetLastError();
+    return launch_following(kern, dim3((unsigned)std::min(want, fit)), (unsigned)threads, 0, 1, st, p);
 }
 
 unsigned unit_grid(long long units, int per_cta) { return (unsigned)((units + per_cta - 1) / per_cta); }
@@ -538,17 +545,15 @@ cudaError_t launch_quant8(int type, const Quant8Params& p, cudaStream_t st) {
     auto kern = type == 0 ? (vec ? quant8_kernel<float, true> : quant8_kernel<float, false>)
                           : (type == 1 ? (vec ? quant8_kernel<__half, true> : quant8_kernel<__half, false>)
                                        : (vec ? quant8_kernel<__nv_bfloat16, true> : quant8_kernel<__nv_bfloat16, false>));
-    kern<<<unit_grid(p.out.rows * p.out.ktiles, kUnitThreads / 32), kUnitThreads, 0, st>>>(p);
-    return cudaGetLastError();
+    return launch_following(kern, dim3(unit_grid(p.out.rows * p.out.ktiles, kUnitThreads / 32)), kUnitThreads, 0, 1, st, p);
 }
 
 cudaError_t launch_quant8_ggml(const void* w, bool q4, long long row_bytes, const Fp8Rows& out, int num_sms,
                                cudaStream_t st) {
     if (out.rows == 0) return cudaSuccess;
     const long long ctas = (out.rows * ((out.K + 127) / 128) * 4 + 127) / 128, cap = (long long)num_sms * 16;
-    quant8_ggml_kernel<<<(unsigned)(ctas < cap ? ctas : cap), 128, 0, st>>>(static_cast<const uint8_t*>(w), q4 ? 1 : 0,
-                                                                            row_bytes, out);
-    return cudaGetLastError();
+    return launch_following(quant8_ggml_kernel, dim3((unsigned)(ctas < cap ? ctas : cap)), 128, 0, 1, st,
+                            static_cast<const uint8_t*>(w), q4 ? 1 : 0, row_bytes, out);
 }
 
 cudaError_t launch_dequant8(int type, const Dequant8Params& p, cudaStream_t st) {
@@ -557,8 +562,7 @@ cudaError_t launch_dequant8(int type, const Dequant8Params& p, cudaStream_t st) 
     auto kern = type == 0 ? (vec ? dequant8_kernel<float, true> : dequant8_kernel<float, false>)
                           : (type == 1 ? (vec ? dequant8_kernel<__half, true> : dequant8_kernel<__half, false>)
                                        : (vec ? dequant8_kernel<__nv_bfloat16, true> : dequant8_kernel<__nv_bfloat16, false>));
-    kern<<<unit_grid(p.in.rows * p.in.ktiles, 2 * kUnitThreads / 32), kUnitThreads, 0, st>>>(p);
-    return cudaGetLastError();
+    return launch_following(kern, dim3(unit_grid(p.in.rows * p.in.ktiles, 2 * kUnitThreads / 32)), kUnitThreads, 0, 1, st, p);
 }
 
 }  // namespace kd

@@ -29,6 +29,33 @@ __device__ __forceinline__ uint32_t fp8_scale_byte(uint32_t amax) {
 __device__ __forceinline__ float fp8_scale_value(uint32_t byte) { return __uint_as_float(byte << 23); }
 __device__ __forceinline__ float fp8_scale_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
 
+// Programmatic launches: a kernel of this path may start while the one before it in the stream runs out, and sets up
+// its barriers, tensor memory and registers meanwhile.  launch_next: the next one may start; called once this CTA holds
+// all that it will ever ask the SM for.  wait_for_previous: everything before in the stream has finished and is visible;
+// every thread calls it before it touches global memory.
+__device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Launches `kern` that way, as clusters of `cluster` CTAs.
+template <typename... P, typename... A>
+cudaError_t launch_following(void (*kern)(P...), dim3 grid, unsigned threads, size_t smem, unsigned cluster, cudaStream_t st,
+                             const A&... args) {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
 // Four values (already divided by the scale, |v| <= 448 or NaN) to e4m3 codes, ties to even; v0 in the low byte.
 __device__ __forceinline__ uint32_t fp8_pack4(float v0, float v1, float v2, float v3) {
     uint32_t r;

@@ -213,6 +213,7 @@ __global__ void __launch_bounds__(kSThreads)
         mbar_init(done, 1);
         *abort_flag = 0;
         fence_mbar_init();
+        wait_for_previous();
         for (int i = 0; i < min(nk, stages); ++i) copy_block(i, i);
     }
     if (warp == 1) {
@@ -223,6 +224,8 @@ __global__ void __launch_bounds__(kSThreads)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *slot;
+    launch_next();
+    wait_for_previous();
 
     if (warp == 0) {
         for (int i = stages; i < nk; ++i) {
@@ -502,6 +505,8 @@ __global__ void __launch_bounds__(kPThreads, 1)
     const uint32_t tmem = *slot;
     const uint32_t full0 = map_to_rank(smem_u32(full), 0);
     const uint32_t acc_read0 = map_to_rank(smem_u32(acc_read), 0);
+    launch_next();
+    wait_for_previous();
 
     auto tile_at = [&](long long t, int& mt, int& nt) {
         const long long band = t / ((long long)kBandM * n_tiles);
@@ -745,8 +750,8 @@ cudaError_t many_typed(const CUtensorMap* tm, const Gemm8Params& p, int num_sms,
         return cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess ? n : 0;
     }();
     if (resident <= 0) return cudaErrorInvalidConfiguration;
-    cfg.gridDim = dim3((unsigned)(2 * (tiles < resident ? tiles : resident)));
-    return cudaLaunchKernelEx(&cfg, kern, tm[0], tm[1], tm[2], tm[3], p);
+    return launch_following(kern, dim3((unsigned)(2 * (tiles < resident ? tiles : resident))), kPThreads, kPSmem, 2, st, tm[0],
+                            tm[1], tm[2], tm[3], p);
 }
 
 template <typename TO>
@@ -755,18 +760,8 @@ cudaError_t few_typed(const CUtensorMap& tmX, const CUtensorMap& tmW, const Gemm
     static std::atomic<unsigned long long> ready{0};
     cudaError_t e = allow_smem(kern, 232448, ready);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)p.splits;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned)((p.N + kGemm8BoxRows - 1) / kGemm8BoxRows) * (unsigned)p.splits);
-    cfg.blockDim = dim3(kSThreads);
-    cfg.dynamicSmemBytes = few_smem(p.nt, ((p.K + 127) / 128 + p.splits - 1) / p.splits);
-    cfg.stream = st;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kern, tmX, tmW, p);
+    return launch_following(kern, dim3((unsigned)((p.N + kGemm8BoxRows - 1) / kGemm8BoxRows) * (unsigned)p.splits), kSThreads,
+                            few_smem(p.nt, ((p.K + 127) / 128 + p.splits - 1) / p.splits), (unsigned)p.splits, st, tmX, tmW, p);
 }
 
 }  // namespace
