@@ -1491,6 +1491,7 @@ kd_attn_status linear_fp8_core(kd_attn_ctx* ctx, const kd_fp8_rows* x, const kd_
     p.y_nb1 = ty.nb1;
     p.y_nb2 = ty.nb2;
     p.y_vec = ty.align >= 32;
+    p.y_pair = (reinterpret_cast<uintptr_t>(y->data) | (uint64_t)ty.nb1 | (uint64_t)ty.nb2) % (2 * elt_size(y->type)) == 0;
     p.L = (int)ty.L;
     p.err = ctx->d_words;
     p.wait_ns = ctx->wait_ns;

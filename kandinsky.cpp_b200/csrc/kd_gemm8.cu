@@ -97,6 +97,18 @@ __device__ __forceinline__ void tmem_ld16_sync(uint32_t taddr, float (&r)[16]) {
     for (int i = 0; i < 16; ++i) r[i] = __uint_as_float(u[i]);
 }
 
+// 32 consecutive columns of 16 TMEM lanes spread over a warp: u[4 k .. 4 k + 1] are columns 8 k + 2 (lane % 4) and the
+// next of lane taddr + lane / 4, u[4 k + 2 .. 4 k + 3] the same columns eight lanes on.
+__device__ __forceinline__ void tmem_ld_spread_sync(uint32_t taddr, uint32_t* u) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;\n"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+          "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+        : "r"(taddr)
+        : "memory");
+}
+
 template <typename T>
 __device__ __forceinline__ T round_to(float v);
 template <>
@@ -431,14 +443,14 @@ __device__ __forceinline__ void st_global_v8(void* p, const uint32_t* u) {
                  "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
                  : "memory");
 }
-// 32 consecutive columns of one row, rounded already (two to a word in 16 bits): n0 is the row's first column here, N
-// the row's length; vec: the rows start on 32-byte boundaries.
+// 32 consecutive columns of one row that starts on a 32-byte boundary, rounded already (two to a word in 16 bits): n0 is
+// the row's first column here, N the row's length.
 template <typename TO>
-__device__ __forceinline__ void store_row32(TO* row, int n0, int N, bool vec, const uint32_t* u) {
+__device__ __forceinline__ void store_row32(TO* row, int n0, int N, const uint32_t* u) {
     constexpr int kW = 32 / sizeof(TO);  // elements of a 32-byte store
 #pragma unroll
     for (int i = 0; i < 32 / kW; ++i) {
-        if (vec && n0 + (i + 1) * kW <= N) {
+        if (n0 + (i + 1) * kW <= N) {
             st_global_v8(row + n0 + i * kW, u + 8 * i);
         } else {
 #pragma unroll
@@ -452,8 +464,7 @@ __device__ __forceinline__ void store_row32(TO* row, int n0, int N, bool vec, co
         }
     }
 }
-
-template <typename TO, int kParts>
+template <typename TO, int kParts, bool kWide>
 __global__ void __launch_bounds__(kPThreads, 1)
     gemm8_many_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                       const __grid_constant__ CUtensorMap tmXs, const __grid_constant__ CUtensorMap tmWs,
@@ -654,7 +665,6 @@ __global__ void __launch_bounds__(kPThreads, 1)
     } else {
         // ------------------------------------------------------------ epilogue: bias, rounding, stores
         const int g = warp / kPGroupWarps;                // the accumulator of this group
-        const int r = ((warp & 3) << 5) + lane;           // token row of this CTA's 128
         const int half = (warp >> 2) & 1, wc = pn / 2;    // columns half * wc .. of the part
         const uint32_t src = tmem + ((uint32_t)((warp & 3) * 32) << 16) + g * kPAccCols + (uint32_t)(half * wc);
         float* bias = reinterpret_cast<float*>(smem + kPBiasAt) + g * 192;
@@ -676,6 +686,9 @@ __global__ void __launch_bounds__(kPThreads, 1)
                                                         mbar_wait(&acc_full[g], uses & 1u, ctl, kErrTimeoutO));
             tc_fence_after();
             ++uses;
+            // kWide, rows on 32-byte boundaries: a lane takes a row.  Other rows are written in pairs of columns, and
+            // lanes that each wrote a row of their own would touch 32 rows with every store (30,952 x 8,194 x 1,382 bf16:
+            // 2,366 us against 412): there four lanes take eight neighbouring columns of a row.
             constexpr int kWords = sizeof(TO) == 4 ? 32 : 16;
             uint32_t u[3 * kWords];
             if (ok) {
@@ -683,16 +696,23 @@ __global__ void __launch_bounds__(kPThreads, 1)
                 for (int c = 0; c < 3; ++c) {
                     if (32 * c < wc) {
                         uint32_t x[32];
-                        tmem_ld32_sync(src + 32 * c, x);
                         const float* b = bias + half * wc + 32 * c;
+                        if constexpr (kWide) {
+                            tmem_ld32_sync(src + 32 * c, x);
+                        } else {
+                            tmem_ld_spread_sync(src + 32 * c, x);
+                            tmem_ld_spread_sync(src + (16u << 16) + 32 * c, x + 16);
+                        }
+                        // value j of a lane: column j, or with four lanes to a row 8 (j / 4 % 4) + 2 (lane % 4) + j % 2
+                        auto sum = [&](int j) {
+                            return __uint_as_float(x[j]) + b[kWide ? j : 8 * (j >> 2 & 3) + 2 * (lane & 3) + (j & 1)];
+                        };
                         if constexpr (sizeof(TO) == 4) {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) u[c * kWords + j] = __float_as_uint(__uint_as_float(x[j]) + b[j]);
+                            for (int j = 0; j < 32; ++j) u[c * kWords + j] = __float_as_uint(sum(j));
                         } else {
 #pragma unroll
-                            for (int j = 0; j < 16; ++j)
-                                u[c * kWords + j] = Pack2<TO>::pack(__uint_as_float(x[2 * j]) + b[2 * j],
-                                                                    __uint_as_float(x[2 * j + 1]) + b[2 * j + 1]);
+                            for (int j = 0; j < 16; ++j) u[c * kWords + j] = Pack2<TO>::pack(sum(2 * j), sum(2 * j + 1));
                         }
                     }
                 }
@@ -700,12 +720,56 @@ __global__ void __launch_bounds__(kPThreads, 1)
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_remote(acc_read0 + 8u * g);
-            const int m = mt * kPairM + (int)rank * kHalfM + r, n = np + half * wc;
-            if (ok && m < p.M) {
-                TO* row = reinterpret_cast<TO*>(token_row(p, m));
+            const int m0 = mt * kPairM + (int)rank * kHalfM + (warp & 3) * 32, n = np + half * wc;
+            if constexpr (kWide) {
+                if (ok && m0 + lane < p.M) {
+                    TO* row = reinterpret_cast<TO*>(token_row(p, m0 + lane));
 #pragma unroll
-                for (int c = 0; c < 3; ++c)
-                    if (32 * c < wc && n + 32 * c < p.N) store_row32(row, n + 32 * c, p.N, p.y_vec, u + c * kWords);
+                    for (int c = 0; c < 3; ++c)
+                        if (32 * c < wc && n + 32 * c < p.N) store_row32(row, n + 32 * c, p.N, u + c * kWords);
+                }
+            } else if (ok) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {  // rows lane / 4 + 8 j of the warp's 32
+                    const int m = m0 + (lane >> 2) + 8 * j;
+                    const bool live = m < p.M;
+                    TO* row = reinterpret_cast<TO*>(token_row(p, live ? m : 0));
+                    // words of two 16-bit columns whose row starts between two words are shifted by one column: each lane
+                    // takes its second column and the first of the next lane's (of the next eight columns' first lane)
+                    const bool shift = sizeof(TO) == 2 && (reinterpret_cast<uintptr_t>(row) & 2u) != 0;
+                    constexpr int kGroups = 12;  // of eight columns
+                    auto word = [&](int g) { return u + (g >> 2) * kWords + (16 * (j >> 1) + 4 * (g & 3) + 2 * (j & 1)) * kWords / 32; };
+#pragma unroll
+                    for (int g = 0; g < kGroups; ++g) {
+                        if (8 * g >= wc) break;
+                        const int col = n + 8 * g + 2 * (lane & 3);
+                        if constexpr (sizeof(TO) == 2) {
+                            const bool last = 8 * (g + 1) >= wc;
+                            const uint32_t mine = *word(g), give = (lane & 3) == 0 && !last ? *word(g + 1 < kGroups ? g + 1 : g) : mine;
+                            const uint32_t next = __shfl_sync(0xffffffffu, give, (lane & ~3) | ((lane + 1) & 3));
+                            uint16_t* r16 = reinterpret_cast<uint16_t*>(row);
+                            if (!live) continue;
+                            if (!shift) {
+                                if (col + 2 <= p.N) *reinterpret_cast<uint32_t*>(r16 + col) = mine;
+                                else if (col < p.N) r16[col] = (uint16_t)mine;
+                            } else {
+                                if (g == 0 && (lane & 3) == 0 && col < p.N) r16[col] = (uint16_t)mine;
+                                if (col + 3 <= p.N && !(last && (lane & 3) == 3))
+                                    *reinterpret_cast<uint32_t*>(r16 + col + 1) = (mine >> 16) | (next << 16);
+                                else if (col + 2 <= p.N) r16[col + 1] = (uint16_t)(mine >> 16);
+                            }
+                        } else if (live) {
+                            const uint32_t* w = word(g);
+                            uint32_t* r32 = reinterpret_cast<uint32_t*>(row);
+                            if (p.y_pair && col + 2 <= p.N) {
+                                *reinterpret_cast<uint2*>(r32 + col) = make_uint2(w[0], w[1]);
+                            } else {
+                                if (col < p.N) r32[col] = w[0];
+                                if (col + 1 < p.N) r32[col + 1] = w[1];
+                            }
+                        }
+                    }
+                }
             }
             __syncwarp();
         }
@@ -726,9 +790,9 @@ __global__ void __launch_bounds__(kPThreads, 1)
     }
 }
 
-template <typename TO, int kParts>
-cudaError_t many_typed(const CUtensorMap* tm, const Gemm8Params& p, int num_sms, cudaStream_t st) {
-    auto kern = gemm8_many_kernel<TO, kParts>;
+template <typename TO, int kParts, bool kWide>
+cudaError_t many_launch(const CUtensorMap* tm, const Gemm8Params& p, int num_sms, cudaStream_t st) {
+    auto kern = gemm8_many_kernel<TO, kParts, kWide>;
     static std::atomic<unsigned long long> ready{0};
     cudaError_t e = allow_smem(kern, kPSmem, ready);
     if (e != cudaSuccess) return e;
@@ -752,6 +816,12 @@ cudaError_t many_typed(const CUtensorMap* tm, const Gemm8Params& p, int num_sms,
     if (resident <= 0) return cudaErrorInvalidConfiguration;
     return launch_following(kern, dim3((unsigned)(2 * (tiles < resident ? tiles : resident))), kPThreads, kPSmem, 2, st, tm[0],
                             tm[1], tm[2], tm[3], p);
+}
+
+template <typename TO>
+cudaError_t many_typed(const CUtensorMap* tm, const Gemm8Params& p, int num_sms, cudaStream_t st) {
+    if (p.y_vec) return p.parts == 2 ? many_launch<TO, 2, true>(tm, p, num_sms, st) : many_launch<TO, 1, true>(tm, p, num_sms, st);
+    return p.parts == 2 ? many_launch<TO, 2, false>(tm, p, num_sms, st) : many_launch<TO, 1, false>(tm, p, num_sms, st);
 }
 
 template <typename TO>
@@ -797,12 +867,9 @@ void gemm8_plan(Gemm8Params* p, int num_sms) {
 
 cudaError_t launch_gemm8(OutType ot, const CUtensorMap* tm, const Gemm8Params& p, int num_sms, cudaStream_t st) {
     if (p.many)
-        return p.parts == 2 ? (ot == OutType::F32 ? many_typed<float, 2>(tm, p, num_sms, st)
-                                                  : (ot == OutType::F16 ? many_typed<__half, 2>(tm, p, num_sms, st)
-                                                                        : many_typed<__nv_bfloat16, 2>(tm, p, num_sms, st)))
-                            : (ot == OutType::F32 ? many_typed<float, 1>(tm, p, num_sms, st)
-                                                  : (ot == OutType::F16 ? many_typed<__half, 1>(tm, p, num_sms, st)
-                                                                        : many_typed<__nv_bfloat16, 1>(tm, p, num_sms, st)));
+        return ot == OutType::F32 ? many_typed<float>(tm, p, num_sms, st)
+                                  : (ot == OutType::F16 ? many_typed<__half>(tm, p, num_sms, st)
+                                                        : many_typed<__nv_bfloat16>(tm, p, num_sms, st));
     return ot == OutType::F32 ? few_typed<float>(tm[0], tm[1], p, st)
                               : (ot == OutType::F16 ? few_typed<__half>(tm[0], tm[1], p, st)
                                                     : few_typed<__nv_bfloat16>(tm[0], tm[1], p, st));

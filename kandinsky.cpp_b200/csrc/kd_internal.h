@@ -236,7 +236,7 @@ struct Gemm8Params {
     int parts;                // many tokens: parts of a tile (1 or 2)
     int splits;               // few tokens: CTAs of a cluster that share a tile's K range
     const float* bias;        // [N] or null
-    bool y_vec;               // 32-byte aligned output rows
+    bool y_vec, y_pair;       // output rows start on 32 bytes; on two elements (f32)
     void* y;                  // token m = l + L * n at y + l * y_nb1 + n * y_nb2
     long long y_nb1, y_nb2;
     int L;                    // at least M when the rows are evenly spaced (y_nb2 is not read)

@@ -269,6 +269,22 @@ def test_linear_strided_output(ctx, kd):
         check_product(t.transpose(0, 1).reshape(N * L, C), x64, w64, f64(bias), dtype)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("C", [1, 63, 130, 193, 383, 577])
+def test_linear_many_tokens_rows_anywhere(ctx, kd, C, dtype):
+    """More tokens than one tile into rows that start on every residue of 32 bytes, odd widths, two sequences."""
+    N, L, K = 2, 333, 200
+    x, x64 = operand(kd, hidden(N * L, K, 61))
+    w, w64 = operand(kd, hidden(C, K, 62) / np.sqrt(K))
+    bias = dev(seeded((C,), 63, 0))
+    for start, pad in ((0, 0), (1, 3), (2, 6), (3, 5), (0, 1)):
+        wide = torch.full((N, L + 1, start + C + pad), 9.0, device="cuda", dtype=TORCH[dtype])
+        y = wide[:, :L, start:start + C]
+        ctx.linear_fp8(x, w, y, bias=bias)
+        check_product(y.reshape(N * L, C), x64, w64, f64(bias), dtype, f"C {C} start {start} pad {pad}")
+        assert (wide[:, :, :start] == 9).all() and (wide[:, :, start + C:] == 9).all() and (wide[:, L] == 9).all()
+
+
 def test_linear_nan_stays_in_its_row(ctx, kd):
     M, N, K = 40, 256, 512
     x, x64 = operand(kd, hidden(M, K, 37))
@@ -346,6 +362,32 @@ def test_streams_and_graph(ctx, kd):
     g.replay()
     check_product(y, fp8_ref.decode(*rows_of(a)), w64, None, "f32")
     assert not torch.equal(y, first)
+    ctx.device_status()
+
+
+def test_back_to_back(ctx, kd):
+    """Launches that may overlap the one before: a chain whose every step reads what the last wrote and writes what the
+    one before read, over buffers used again at once, gives what the same chain gives with a wait after every call."""
+    M, C = 300, 640
+    ws = [operand(kd, hidden(C, C, 70 + i) / np.sqrt(C))[0] for i in range(2)]
+    x0 = dev(hidden(M, C, 72), "bf16")
+
+    def chain(sync, m):
+        x, y, h = x0[:m].clone(), torch.empty(m, C, device="cuda", dtype=torch.bfloat16), torch.empty(m, C, device="cuda", dtype=torch.bfloat16)
+        a = kd.Fp8Rows.empty(m, C)
+        for i in range(40):
+            for call in (lambda: ctx.rms_norm_fp8(x, a, residual=y if i else None, h=h), lambda: ctx.linear_fp8(a, ws[i & 1], y),
+                         lambda: ctx.quantize_fp8(y, a), lambda: ctx.linear_fp8(a, ws[1 - (i & 1)], x),
+                         lambda: ctx.dequantize_fp8(a, h), lambda: x.add_(h)):
+                call()
+                if sync:
+                    torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return x, y, h, *rows_of(a)
+
+    for m in (3, 200, M):
+        for p, q in zip(chain(False, m), chain(True, m)):
+            assert torch.equal(p, q) if isinstance(p, torch.Tensor) else np.array_equal(p, q)
     ctx.device_status()
 
 
