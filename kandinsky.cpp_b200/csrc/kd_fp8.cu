@@ -8,7 +8,9 @@
 // All of them move bytes and do little else: each value is read once and written once, held in registers between.
 // A warp's unit of work is 512 columns of a row: four blocks, one 32-bit word of scale bytes, sixteen columns a lane.
 // Where rows start on 16-byte boundaries a lane holds sixteen consecutive columns and moves them in wide accesses;
-// elsewhere (odd row lengths) lane l holds columns l, l + 32, ..., so that its narrow accesses are still coalesced.
+// elsewhere (odd row lengths) lane l holds the pairs of columns 2 l, 2 l + 64, ..., so that its narrow accesses are still
+// coalesced.  16-bit rows that start between two words are moved word by word all the same, shifted by one column:
+// the missing half comes from the next lane.
 #include <algorithm>
 #include <type_traits>
 
@@ -126,14 +128,100 @@ __device__ __forceinline__ void scale16(float (&v)[kPer], float s) {
 // The column of value j of a lane in the chunk from c0.
 template <bool kVec>
 __device__ __forceinline__ int column(int c0, int lane, int j) {
-    return kVec ? c0 + lane * kPer + j : c0 + j * 32 + lane;
+    return kVec ? c0 + lane * kPer + j : c0 + 64 * (j >> 1) + 2 * lane + (j & 1);
+}
+
+// The second half of a lane's word and the first of the word after it, which the next lane has, or lane 0 as its next.
+__device__ __forceinline__ uint32_t shifted(uint32_t mine, uint32_t lane0_next, int lane) {
+    const uint32_t next = __shfl_sync(kAll, lane == 0 ? lane0_next : mine, (lane + 1) & 31);
+    return (mine >> 16) | (next << 16);
+}
+
+// A lane's pairs of columns of a row of K from anywhere, zeros at and past K.
+template <typename T>
+__device__ __forceinline__ void load_pairs(const T* row, int c0, int lane, int K, Raw<T>& a) {
+    if constexpr (sizeof(T) == 4) {
+        const bool pair = (reinterpret_cast<uintptr_t>(row) & 7u) == 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int c = column<false>(c0, lane, 2 * i);
+            const uint32_t* p = reinterpret_cast<const uint32_t*>(row) + c;
+            uint2 u = make_uint2(0, 0);
+            if (pair && c + 2 <= K) {
+                u = *reinterpret_cast<const uint2*>(p);
+            } else {
+                if (c < K) u.x = p[0];
+                if (c + 1 < K) u.y = p[1];
+            }
+            a.w[2 * i] = u.x;
+            a.w[2 * i + 1] = u.y;
+        }
+    } else {
+        const uint16_t* r = reinterpret_cast<const uint16_t*>(row);
+        if ((reinterpret_cast<uintptr_t>(row) & 2u) == 0) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int c = column<false>(c0, lane, 2 * i);
+                a.w[i] = c + 2 <= K ? *reinterpret_cast<const uint32_t*>(r + c) : (c < K ? r[c] : 0u);
+            }
+        } else {
+            uint32_t w[9];  // columns c - 1 and c: the ones that share a word
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int c = column<false>(c0, lane, 2 * i);
+                if (c == 0) w[i] = (uint32_t)r[0] << 16;
+                else w[i] = c < K ? *reinterpret_cast<const uint32_t*>(r + c - 1) : (c - 1 < K ? r[c - 1] : 0u);
+            }
+            w[8] = lane == 0 && c0 + kChunk - 1 < K ? r[c0 + kChunk - 1] : 0u;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a.w[i] = shifted(w[i], w[i + 1], lane);
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store_pairs(T* row, int c0, int lane, int K, const Raw<T>& a) {
+    if constexpr (sizeof(T) == 4) {
+        const bool pair = (reinterpret_cast<uintptr_t>(row) & 7u) == 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int c = column<false>(c0, lane, 2 * i);
+            uint32_t* p = reinterpret_cast<uint32_t*>(row) + c;
+            if (pair && c + 2 <= K) {
+                *reinterpret_cast<uint2*>(p) = make_uint2(a.w[2 * i], a.w[2 * i + 1]);
+            } else {
+                if (c < K) p[0] = a.w[2 * i];
+                if (c + 1 < K) p[1] = a.w[2 * i + 1];
+            }
+        }
+    } else {
+        uint16_t* r = reinterpret_cast<uint16_t*>(row);
+        if ((reinterpret_cast<uintptr_t>(row) & 2u) == 0) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int c = column<false>(c0, lane, 2 * i);
+                if (c + 2 <= K) *reinterpret_cast<uint32_t*>(r + c) = a.w[i];
+                else if (c < K) r[c] = (uint16_t)a.w[i];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int c = column<false>(c0, lane, 2 * i);
+                const uint32_t u = shifted(a.w[i], a.w[i < 7 ? i + 1 : i], lane);  // columns c + 1 and c + 2
+                if (i == 0 && lane == 0 && c < K) r[c] = (uint16_t)a.w[0];
+                if (c + 3 <= K && !(i == 7 && lane == 31)) *reinterpret_cast<uint32_t*>(r + c + 1) = u;
+                else if (c + 2 <= K) r[c + 1] = (uint16_t)u;
+            }
+        }
+    }
 }
 
 // A lane's sixteen values of a row of K, zeros at and past K.  align: of the row, in bytes (32, 16 or less).
 template <typename T, bool kVec>
 __device__ __forceinline__ void load16(const T* row, int c0, int lane, int K, int align, Raw<T>& a) {
     constexpr int kW = Raw<T>::kWords;
-    if (kVec && column<kVec>(c0, lane, kPer) <= K) {
+    if constexpr (!kVec) {
+        load_pairs(row, c0, lane, K, a);
+    } else if (column<kVec>(c0, lane, kPer) <= K) {
         const T* p = row + column<kVec>(c0, lane, 0);
         if (align >= 32) {
 #pragma unroll
@@ -156,7 +244,9 @@ __device__ __forceinline__ void load16(const T* row, int c0, int lane, int K, in
 template <typename T, bool kVec>
 __device__ __forceinline__ void store16(T* row, int c0, int lane, int K, int align, const Raw<T>& a) {
     constexpr int kW = Raw<T>::kWords;
-    if (kVec && column<kVec>(c0, lane, kPer) <= K) {
+    if constexpr (!kVec) {
+        store_pairs(row, c0, lane, K, a);
+    } else if (column<kVec>(c0, lane, kPer) <= K) {
         T* p = row + column<kVec>(c0, lane, 0);
         if (align >= 32) {
 #pragma unroll
@@ -237,9 +327,9 @@ __device__ __forceinline__ void encode16(float (&v)[kPer], const Fp8Rows& o, lon
             const float inv = fp8_scale_inverse(byte);
             const uint32_t u = fp8_pack4(v[4 * b] * inv, v[4 * b + 1] * inv, v[4 * b + 2] * inv, v[4 * b + 3] * inv);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int c = column<kVec>(c0, lane, 4 * b + i);
-                if (c < o.Kp) codes[c] = (uint8_t)(u >> (8 * i));
+            for (int i = 0; i < 2; ++i) {
+                const int c = column<kVec>(c0, lane, 4 * b + 2 * i);
+                if (c < o.Kp) *reinterpret_cast<uint16_t*>(codes + c) = (uint16_t)(u >> (16 * i));
             }
         }
     }
@@ -480,9 +570,9 @@ __global__ void __launch_bounds__(kUnitThreads) dequant8_kernel(const Dequant8Pa
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < kPer; ++j)
+            for (int j = 0; j < kPer; j += 2)
                 if (column<kVec>(c0[u], lane, j) < p.in.K)
-                    codes[u][j >> 2] |= (uint32_t)src[column<kVec>(c0[u], lane, j)] << (8 * (j & 3));
+                    codes[u][j >> 2] |= (uint32_t)*reinterpret_cast<const uint16_t*>(src + column<kVec>(c0[u], lane, j)) << (8 * (j & 2));
         }
     }
 #pragma unroll

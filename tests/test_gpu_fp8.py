@@ -95,6 +95,34 @@ def test_quantize_strided_and_misaligned(ctx, kd):
             assert (y[:, :, :3] == 7).all() and (y[:, :, 3 + K:] == 7).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("K", [1, 2, 63, 129, 511, 512, 513, 1023, 1025, 1537])
+def test_rows_that_start_anywhere(ctx, kd, K, dtype):
+    """Quantising, the norm with residual and h, and reading back, on rows that start on every residue of 16 bytes."""
+    R = 9
+    for start, pad in ((0, 1), (1, 0), (1, 1), (3, 2), (2, 4)):
+        def place(v):
+            wide = torch.full((R, start + K + pad), 5.0, device="cuda", dtype=TORCH[dtype])
+            wide[:, start:start + K] = v
+            return wide, wide[:, start:start + K]
+        _, x = place(dev(hidden(R, K, 14), dtype))
+        _, res = place(dev(seeded((R, K), 15, 0), dtype))
+        r = kd.Fp8Rows.empty(R, K)
+        ctx.quantize_fp8(x, r)
+        codes, s = fp8_ref.encode(f64(x))
+        got, gs = rows_of(r)
+        assert np.array_equal(gs, s) and np.array_equal(got, codes)
+        wy, y = place(0.0)
+        ctx.dequantize_fp8(r, y)
+        assert np.array_equal(f64(y), fp8_ref.round_to(fp8_ref.decode(codes, s), dtype))
+        wh, h = place(0.0)
+        ctx.rms_norm_fp8(x, r, residual=res, h=h)
+        assert torch.equal(h, (x.float() + res.float()).to(TORCH[dtype]))
+        check_norm(kd, r, f64(h), None, 1e-6)
+        for w in (wy, wh):
+            assert (w[:, :start] == 5).all() and (w[:, start + K:] == 5).all()
+
+
 def test_quantize_edges(ctx, kd):
     """Zeros, the scale's border (448 * 2^e and one step above), subnormal inputs, NaN and infinities; codes and
     scales outside the rows stay as they were."""
