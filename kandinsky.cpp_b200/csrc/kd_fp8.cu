@@ -47,6 +47,8 @@ template <typename T>
 struct Raw {
     static constexpr int kWords = sizeof(T) * kPer / 4;
     uint32_t w[kWords];
+    uint32_t more;  // load_pairs: half a word past them, in lane 0
+    bool shift;     // load_pairs: the words still start one column early (settle)
 };
 __device__ __forceinline__ void ld_v8(const void* p, uint32_t* w) {
     asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
@@ -137,7 +139,8 @@ __device__ __forceinline__ uint32_t shifted(uint32_t mine, uint32_t lane0_next, 
     return (mine >> 16) | (next << 16);
 }
 
-// A lane's pairs of columns of a row of K from anywhere, zeros at and past K.
+// A lane's pairs of columns of a row of K from anywhere, zeros at and past K; settle() puts them in place (apart, so that
+// loads can be under way for long: the shift would wait for them).
 template <typename T>
 __device__ __forceinline__ void load_pairs(const T* row, int c0, int lane, int K, Raw<T>& a) {
     if constexpr (sizeof(T) == 4) {
@@ -165,17 +168,24 @@ __device__ __forceinline__ void load_pairs(const T* row, int c0, int lane, int K
                 a.w[i] = c + 2 <= K ? *reinterpret_cast<const uint32_t*>(r + c) : (c < K ? r[c] : 0u);
             }
         } else {
-            uint32_t w[9];  // columns c - 1 and c: the ones that share a word
+            // columns c - 1 and c: the ones that share a word
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int c = column<false>(c0, lane, 2 * i);
-                if (c == 0) w[i] = (uint32_t)r[0] << 16;
-                else w[i] = c < K ? *reinterpret_cast<const uint32_t*>(r + c - 1) : (c - 1 < K ? r[c - 1] : 0u);
+                if (c == 0) a.w[i] = (uint32_t)r[0] << 16;
+                else a.w[i] = c < K ? *reinterpret_cast<const uint32_t*>(r + c - 1) : (c - 1 < K ? r[c - 1] : 0u);
             }
-            w[8] = lane == 0 && c0 + kChunk - 1 < K ? r[c0 + kChunk - 1] : 0u;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) a.w[i] = shifted(w[i], w[i + 1], lane);
+            a.more = lane == 0 && c0 + kChunk - 1 < K ? r[c0 + kChunk - 1] : 0u;
         }
+        a.shift = (reinterpret_cast<uintptr_t>(row) & 2u) != 0;
+    }
+}
+template <typename T, bool kVec>
+__device__ __forceinline__ void settle(Raw<T>& a, int lane) {
+    if constexpr (!kVec && sizeof(T) == 2) {
+        if (!a.shift) return;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a.w[i] = shifted(a.w[i], i < 7 ? a.w[i + 1] : a.more, lane);
     }
 }
 template <typename T>
@@ -409,6 +419,8 @@ __global__ void __launch_bounds__(kMaxThreads, std::max(1, norm_threads<T>() / k
         uint64_t sums = f2_pack(0.0f, 0.0f);
 #pragma unroll
         for (int q = 0; q < kChunks; ++q) {
+            settle<T, kVec>(x[q], lane);
+            if (p.r) settle<T, kVec>(r[q], lane);
             // the sum is rounded to the rows' type, as it is stored, and the norm is of the stored value
             if (p.r) add_rows(x[q], r[q]);
             if (p.h)
@@ -469,6 +481,7 @@ __global__ void __launch_bounds__(kUnitThreads) quant8_kernel(const Quant8Params
     Raw<T> a;
     load16<T, kVec>(row_at(static_cast<const T*>(p.x), row, p.L >= p.out.rows, p.L, p.x_nb1, p.x_nb2), chunk * kChunk, lane, p.out.K,
                     p.align, a);
+    settle<T, kVec>(a, lane);
     float v[kPer];
     widen(a, v);
     encode16<kVec>(v, p.out, row, chunk * kChunk, lane);
