@@ -1370,7 +1370,7 @@ kd_attn_status quantize_weight_fp8_core(kd_attn_ctx* ctx, const kd_linear* w, kd
     if (o.rows && !w->data) return fail(ctx, KD_ATTN_ERR_INVALID_ARGUMENT, "weight data is NULL");
     if (reinterpret_cast<uintptr_t>(w->data) % 2 || w->nb1 % 2)
         return fail(ctx, KD_ATTN_ERR_UNSUPPORTED, "weight blocks must be 2-byte aligned");
-    KD_CUDA(ctx, launch_quant8_ggml(w->data, w->type == KD_ATTN_TYPE_Q4_0, (long long)w->nb1, o, ctx->num_sms, st));
+    KD_CUDA(ctx, launch_quant8_ggml(w->data, w->type == KD_ATTN_TYPE_Q4_0, (long long)w->nb1, o, st));
     return KD_ATTN_OK;
 }
 

@@ -487,69 +487,72 @@ __global__ void __launch_bounds__(kUnitThreads) quant8_kernel(const Quant8Params
     encode16<kVec>(v, p.out, row, chunk * kChunk, lane);
 }
 
-// Weight rows of 32-element ggml blocks (q8_0: f16 scale and 32 int8; q4_0: f16 scale and 16 bytes, element j in
-// the low nibble, j + 16 in the high one): four lanes per block of 128, one ggml block each.  Blocks are 34 or 18
-// bytes long, so a lane reads 16-bit words.
-__global__ void quant8_ggml_kernel(const uint8_t* w, int q4, long long row_bytes, const Fp8Rows o) {
-    const int blocks = (o.K + 127) >> 7;
-    const long long total = o.rows * blocks;
+// Weight rows of 32-element ggml blocks (q8_0: f16 scale d and 32 int8; q4_0: f16 scale d and 16 bytes, element j in the
+// low nibble, j + 16 in the high one, less 8): a lane per ggml block, four to a block of 128, 1,024 columns a warp.
+// Blocks are 34 or 18 bytes long, so a lane reads 16-bit words.  (Bringing the warp's bytes into shared memory in
+// 16-byte loads first was slower, 13.6 us against 11.0 for 4,096 x 4,096 q8_0: instructions bound it.)  So the codes q
+// become f32 by their place in a significand, the largest is found among them, and d and the new scale, a power of
+// two, are multiplied once: d * q * 2^-e is exact whichever comes first (11 and 8 significant bits).
+constexpr int kGgmlWarps = 4;
+template <bool kQ4>
+__global__ void __launch_bounds__(32 * kGgmlWarps) quant8_ggml_kernel(const uint8_t* w, long long row_bytes, const Fp8Rows o) {
+    constexpr int kBytes = kQ4 ? 18 : 34;
+    constexpr float kBias = 8388608.0f + (kQ4 ? 8.0f : 128.0f);  // 2^23, and what the codes are raised by
+    const int lane = threadIdx.x & 31;
+    const int chunks = (o.K + 1023) >> 10;
+    const long long unit = (long long)blockIdx.x * kGgmlWarps + (threadIdx.x >> 5), units = o.rows * chunks;
     launch_next();
     wait_for_previous();
-    const long long step = ((long long)gridDim.x * blockDim.x) >> 2;
-    for (long long i = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 2; (i & ~7ll) < total; i += step) {
-        const bool live = i < total;
-        const long long row = (live ? i : total - 1) / blocks;
-        const int c = (int)((live ? i : total - 1) % blocks) * 128 + (threadIdx.x & 3) * 32;
-        float v[32];
+    if (unit >= units) return;
+    long long row;
+    int chunk;
+    unit_at(unit, chunks, units <= 0xffffffffll, row, chunk);
+    const int c = chunk * 1024 + lane * 32;
+    const bool live = c < o.K;  // (K is a multiple of 32: a ggml block is wholly inside)
+    const uint16_t* b = reinterpret_cast<const uint16_t*>(w + row * row_bytes + (long long)(live ? c >> 5 : 0) * kBytes);
+    float d = live ? __half2float(__ushort_as_half(b[0])) : 0.0f;
+    float q[32];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-        if (c < o.K) {
-            const uint16_t* b =
-                reinterpret_cast<const uint16_t*>(w + row * row_bytes + (long long)(c >> 5) * (q4 ? 18 : 34));
-            const float d = __half2float(__ushort_as_half(b[0]));
-            if (q4) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const unsigned u = b[1 + j];
-                    v[2 * j] = d * (float)((int)(u & 15u) - 8);
-                    v[2 * j + 16] = d * (float)((int)((u >> 4) & 15u) - 8);
-                    v[2 * j + 1] = d * (float)((int)((u >> 8) & 15u) - 8);
-                    v[2 * j + 17] = d * (float)((int)(u >> 12) - 8);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const unsigned u = b[1 + j];
-                    v[2 * j] = d * (float)(int8_t)(u & 255u);
-                    v[2 * j + 1] = d * (float)(int8_t)(u >> 8);
-                }
-            }
+    for (int j = 0; j < (kQ4 ? 8 : 16); ++j) {
+        const uint32_t u = live ? b[1 + j] : 0u;
+        if constexpr (kQ4) {
+            q[2 * j] = __uint_as_float(0x4B000000u | (u & 15u)) - kBias;
+            q[2 * j + 16] = __uint_as_float(0x4B000000u | (u >> 4 & 15u)) - kBias;
+            q[2 * j + 1] = __uint_as_float(0x4B000000u | (u >> 8 & 15u)) - kBias;
+            q[2 * j + 17] = __uint_as_float(0x4B000000u | (u >> 12)) - kBias;
+        } else {
+            const uint32_t r = u ^ 0x8080u;
+            q[2 * j] = __uint_as_float(__byte_perm(r, 0x4B000000u, 0x7650)) - kBias;
+            q[2 * j + 1] = __uint_as_float(__byte_perm(r, 0x4B000000u, 0x7651)) - kBias;
         }
-        uint32_t top = 0;
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            const uint32_t a = __float_as_uint(fabsf(v[j]));
-            if (a >= kInfBits) v[j] = __uint_as_float(0x7FFFFFFFu);  // a block whose f16 scale is not finite
-            else top = max(top, a);
-        }
-#pragma unroll
-        for (int s = 2; s; s >>= 1) top = max(top, __shfl_xor_sync(kAll, top, s));
-        const uint32_t byte = fp8_scale_byte(top);
-        const float inv = fp8_scale_inverse(byte);
-        if (!live || c >= o.K) continue;  // (K is a multiple of 32: a ggml block is wholly inside)
-        uint4* dst = reinterpret_cast<uint4*>(o.codes + row * o.row_bytes + c);
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            uint32_t u[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float* a = v + 16 * q + 4 * j;
-                u[j] = fp8_pack4(a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
-            }
-            dst[q] = make_uint4(u[0], u[1], u[2], u[3]);
-        }
-        if ((c & 127) == 0) o.scales[fp8_scale_offset(row, c >> 7, o.ktiles)] = (uint8_t)byte;
     }
+    float most = fmaxf(fabsf(q[0]), fabsf(q[1]));
+#pragma unroll
+    for (int j = 2; j < 32; j += 2) most = fmax3(most, fabsf(q[j]), fabsf(q[j + 1]));
+    uint32_t top = __float_as_uint(fabsf(d) * most);
+    // a ggml block whose scale is not finite is NaN (its zeros too, 0 * d) and does not count
+    const bool nan = (__float_as_uint(d) & kInfBits) == kInfBits;
+    if (nan) top = 0;
+#pragma unroll
+    for (int s = 2; s; s >>= 1) top = max(top, __shfl_xor_sync(kAll, top, s));
+    const uint32_t byte = fp8_scale_byte(top);
+    if (!live) return;
+    d = nan ? __uint_as_float(0x7FFFFFFFu) : d * fp8_scale_inverse(byte);
+    uint4* dst = reinterpret_cast<uint4*>(o.codes + row * o.row_bytes + c);
+    const uint64_t dd = f2_pack(d, d);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        uint32_t u[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float* a = q + 16 * i + 4 * j;
+            f2_unpack(mul_f32x2(f2_pack(a[0], a[1]), dd), a[0], a[1]);
+            f2_unpack(mul_f32x2(f2_pack(a[2], a[3]), dd), a[2], a[3]);
+            u[j] = fp8_pack4(a[0], a[1], a[2], a[3]);
+        }
+        dst[i] = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+    if ((lane & 3) == 0) o.scales[fp8_scale_offset(row, c >> 7, o.ktiles)] = (uint8_t)byte;
 }
 
 // Two units a warp: their loads are under way together.
@@ -651,12 +654,11 @@ cudaError_t launch_quant8(int type, const Quant8Params& p, cudaStream_t st) {
     return launch_following(kern, dim3(unit_grid(p.out.rows * p.out.ktiles, kUnitThreads / 32)), kUnitThreads, 0, 1, st, p);
 }
 
-cudaError_t launch_quant8_ggml(const void* w, bool q4, long long row_bytes, const Fp8Rows& out, int num_sms,
-                               cudaStream_t st) {
+cudaError_t launch_quant8_ggml(const void* w, bool q4, long long row_bytes, const Fp8Rows& out, cudaStream_t st) {
     if (out.rows == 0) return cudaSuccess;
-    const long long ctas = (out.rows * ((out.K + 127) / 128) * 4 + 127) / 128, cap = (long long)num_sms * 16;
-    return launch_following(quant8_ggml_kernel, dim3((unsigned)(ctas < cap ? ctas : cap)), 128, 0, 1, st,
-                            static_cast<const uint8_t*>(w), q4 ? 1 : 0, row_bytes, out);
+    return launch_following(q4 ? quant8_ggml_kernel<true> : quant8_ggml_kernel<false>,
+                            dim3(unit_grid(out.rows * ((out.K + 1023) / 1024), kGgmlWarps)), 32 * kGgmlWarps, 0, 1, st,
+                            static_cast<const uint8_t*>(w), row_bytes, out);
 }
 
 cudaError_t launch_dequant8(int type, const Dequant8Params& p, cudaStream_t st) {

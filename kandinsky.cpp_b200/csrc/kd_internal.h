@@ -221,8 +221,7 @@ constexpr int kNorm8MaxCols = 32768;
 cudaError_t launch_norm8(int type, const Norm8Params& p, int num_sms, cudaStream_t st);
 cudaError_t launch_quant8(int type, const Quant8Params& p, cudaStream_t st);
 // q8_0 (or q4_0) weight rows row_bytes apart, 2-byte aligned; out.K a multiple of 32.
-cudaError_t launch_quant8_ggml(const void* w, bool q4, long long row_bytes, const Fp8Rows& out, int num_sms,
-                               cudaStream_t st);
+cudaError_t launch_quant8_ggml(const void* w, bool q4, long long row_bytes, const Fp8Rows& out, cudaStream_t st);
 cudaError_t launch_dequant8(int type, const Dequant8Params& p, cudaStream_t st);
 
 // y[m][n] = sum_k x[m][k] w[n][k] + bias[n] of two 8-bit operands (kd_gemm8.cu).

@@ -154,7 +154,7 @@ def test_quantize_edges(ctx, kd):
 
 
 @pytest.mark.parametrize("name", ["q8_0", "q4_0", "f16", "bf16", "f32"])
-@pytest.mark.parametrize("C,K", [(5, 32), (64, 416), (129, 1024)])
+@pytest.mark.parametrize("C,K", [(5, 32), (64, 416), (129, 1024), (33, 4096), (7, 1536), (9, 2080)])
 def test_quantize_weight(ctx, kd, name, C, K):
     w = (seeded((C, K), 13, 0) / np.sqrt(K)).astype(np.float32)
     wtype = {"q8_0": kd.Q8_0, "q4_0": kd.Q4_0, "f16": kd.F16, "bf16": kd.BF16, "f32": kd.F32}[name]
@@ -172,6 +172,25 @@ def test_quantize_weight(ctx, kd, name, C, K):
     assert np.array_equal(gs, s)
     # a ggml zero may be -0 * d
     assert np.array_equal(fp8_ref.VALUES[got], fp8_ref.VALUES[codes])
+
+
+def test_quantize_ggml_edges(ctx, kd):
+    """ggml blocks with scales of zero, negative, subnormal, infinite and NaN, and the extreme codes."""
+    K, C = 256, 6
+    raw = np.zeros((C, K // 32, 34), np.uint8)
+    raw[:, :, 2:] = np.arange(32, dtype=np.uint8) * 8 + np.arange(K // 32, dtype=np.uint8)[:, None]  # all of int8 among them
+    d = np.full((C, K // 32), 0.01, np.float16)
+    d[0, 1], d[1, :4], d[2, 2], d[3, 5], d[4, 6] = -0.5, 0.0, 6e-8, np.inf, np.nan
+    raw[:, :, :2] = d.view(np.uint8).reshape(C, K // 32, 2)
+    with np.errstate(invalid="ignore"):
+        v = (d[:, :, None].astype(np.float64) * raw[:, :, 2:].view(np.int8)).reshape(C, K)
+    codes, s = fp8_ref.encode(v)
+    r = kd.Fp8Rows.empty(C, K)
+    t = torch.from_numpy(raw.reshape(C, -1)).cuda()
+    ctx.quantize_weight_fp8(kd.KdLinear.of(t, kd.Q8_0, K, C), r)
+    got, gs = rows_of(r)
+    assert np.array_equal(gs, s)
+    assert np.array_equal(fp8_ref.VALUES[got], fp8_ref.VALUES[codes], equal_nan=True)
 
 
 # ------------------------------------------------------------------ norm
