@@ -311,14 +311,19 @@ __device__ __forceinline__ void block_tops(float (&v)[kPer], uint32_t (&top)[4])
     }
 }
 
+// A value within kNear steps of f32 of the middle between two (normal) codes, where its last bits decide, gives at most
+// kMiddle: the 20 fraction bits that a code drops, around one half, shifted up by 12.
+constexpr uint32_t kNear = 12, kMiddle = 2 * kNear << 12;
+__device__ __forceinline__ uint32_t middle(float v) { return (__float_as_uint(v) << 12) + ((kNear - 0x80000u) << 12); }
+
 // 512 columns of a row from c0, sixteen values to a lane (zeros past K), into codes and scale bytes.  All lanes take
-// part.
-template <bool kVec>
-__device__ __forceinline__ void encode16(float (&v)[kPer], const Fp8Rows& o, long long row, int c0, int lane) {
+// part.  kAgain: the values have been rounded to f32, and a code of one near a middle may be the wrong neighbour;
+// returns which of the lane's values are (bit j), and the scale bytes.
+template <bool kVec, bool kAgain>
+__device__ __forceinline__ uint32_t encode16(float (&v)[kPer], const Fp8Rows& o, long long row, int c0, int lane, uint32_t& word) {
     uint32_t top[4];
     block_tops<kVec>(v, top);
     uint8_t* codes = o.codes + row * o.row_bytes;
-    uint32_t word;  // the scale bytes of the four blocks
     if constexpr (kVec) {
         const uint32_t byte = fp8_scale_byte(top[0]);
         word = __reduce_or_sync(kAll, byte << (8 * (lane >> 3)));
@@ -335,7 +340,9 @@ __device__ __forceinline__ void encode16(float (&v)[kPer], const Fp8Rows& o, lon
             const uint32_t byte = fp8_scale_byte(top[b]);
             word |= byte << (8 * b);
             const float inv = fp8_scale_inverse(byte);
-            const uint32_t u = fp8_pack4(v[4 * b] * inv, v[4 * b + 1] * inv, v[4 * b + 2] * inv, v[4 * b + 3] * inv);
+#pragma unroll
+            for (int i = 4 * b; i < 4 * b + 4; ++i) v[i] *= inv;
+            const uint32_t u = fp8_pack4(v[4 * b], v[4 * b + 1], v[4 * b + 2], v[4 * b + 3]);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int c = column<kVec>(c0, lane, 4 * b + 2 * i);
@@ -349,6 +356,17 @@ __device__ __forceinline__ void encode16(float (&v)[kPer], const Fp8Rows& o, lon
     } else if (lane < 4 && c0 + lane * 128 < o.K) {  // bytes of blocks past K stay as they were
         s[lane] = (uint8_t)(word >> (8 * lane));
     }
+    uint32_t near = 0;
+    if constexpr (kAgain) {
+        uint32_t least = middle(v[0]);
+#pragma unroll
+        for (int j = 1; j + 1 < kPer; j += 2) least = __vimin3_u32(least, middle(v[j]), middle(v[j + 1]));
+        if (min(least, middle(v[kPer - 1])) <= kMiddle) {
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) near |= middle(v[j]) <= kMiddle ? 1u << j : 0u;
+        }
+    }
+    return near;
 }
 
 // (row, 512-column chunk) of a warp's unit; 32-bit arithmetic where the units allow it.
@@ -376,14 +394,57 @@ __device__ __forceinline__ P* row_at(P* base, long long m, bool even, long long 
 template <typename T>
 constexpr int norm_threads() { return sizeof(T) == 2 ? 768 : 512; }
 
+// The sum over a warp of values >= 0, to 2^-26 of the largest: in whole numbers, which one instruction adds exactly
+// (in f32 the five rounded steps would be off by as much as a value's own rounding, and move every value of the row
+// across the middles between codes).  NaN if any is, infinite if any is.
+__device__ __forceinline__ double warp_sum(float v) {
+    const uint32_t top = __reduce_max_sync(kAll, __float_as_uint(v) & 0x7FFFFFFFu);
+    if (top >= kInfBits) return __uint_as_float(top);
+    const float lift = top < (64u << 23) ? 0x1p64f : 1.0f;             // so that the factor below is a normal number
+    const uint32_t e = __float_as_uint(__uint_as_float(top) * lift) >> 23;  // lifted values are below 2^(e - 126)
+    const float unit = __uint_as_float((279u - e) << 23);              // 2^(152 - e): below 2^26
+    const uint32_t total = __reduce_add_sync(kAll, __float2uint_rn(v * lift * unit));
+    return (double)total * (1.0 / lift) * __hiloint2double((int)((e + (1023u - 152u)) << 20), 0);
+}
+
+// The codes of some of a lane's values (bit j of `near`) once more, from the row in memory and in 64 bits: the value in
+// units of its scale, truncated to f32 with the last bit set if anything was dropped, which rounds as the value does.
+template <typename T, bool kVec>
+__device__ __forceinline__ void encode_again(const Norm8Params& p, long long m, int c0, int lane, uint32_t near, uint32_t word,
+                                             double squares) {
+    const bool even = p.L >= p.out.rows;
+    const double inv = 1.0 / sqrt(squares / p.out.K + p.eps);
+    for (; near; near &= near - 1) {
+        const int j = __ffs(near) - 1, c = column<kVec>(c0, lane, j);
+        if (c >= p.out.K) break;
+        float h;
+        if (p.h) {
+            h = to_f32(row_at(static_cast<const T*>(p.h), m, even, p.L, p.h_nb1, p.h_nb2)[c]);
+        } else {
+            T a = row_at(static_cast<const T*>(p.x), m, even, p.L, p.x_nb1, p.x_nb2)[c];
+            if (p.r) {
+                const T b = row_at(static_cast<const T*>(p.r), m, even, p.L, p.r_nb1, p.r_nb2)[c];
+                if constexpr (sizeof(T) == 4) a = __fadd_rn(a, b);
+                else a = __hadd(a, b);
+            }
+            h = to_f32(a);
+        }
+        const uint32_t byte = word >> (8 * (kVec ? lane >> 3 : j >> 2)) & 255u;
+        const double v = h * inv * (p.gain ? p.gain[c] : 1.0f) * fp8_scale_inverse(byte);
+        float f = __double2float_rz(v);
+        if ((double)f != v) f = __uint_as_float(__float_as_uint(f) | 1u);
+        p.out.codes[m * p.out.row_bytes + c] = (uint8_t)fp8_pack4(f, 0.0f, 0.0f, 0.0f);
+    }
+}
+
 // One row at a time by the CTA (kWarpRows: by each warp of its own), a warp holding one chunk of 512 columns, or two
 // in CTAs of more than 512 threads.  The CTA stays and takes every gridDim.x-th row: the gain is read once, and
 // the next row is on its way (in registers) while this one is summed, divided and written.  One pass over the data.
 template <typename T, bool kVec, int kMaxThreads, bool kWarpRows>
-__global__ void __launch_bounds__(kMaxThreads, std::max(1, norm_threads<T>() / kMaxThreads)) norm8_kernel(const Norm8Params p) {
+__global__ void __launch_bounds__(kMaxThreads, std::max(1, norm_threads<T>() / kMaxThreads)) norm8_kernel(const __grid_constant__ Norm8Params p) {
     constexpr int kChunks = kMaxThreads > 512 ? 2 : 1;
     constexpr bool kAhead = kChunks == 1;  // a second row of 32 columns a thread does not fit the registers
-    __shared__ float part[2][32];
+    __shared__ double part[2][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int K = p.out.K;
     launch_next();
@@ -423,9 +484,11 @@ __global__ void __launch_bounds__(kMaxThreads, std::max(1, norm_threads<T>() / k
             if (p.r) settle<T, kVec>(r[q], lane);
             // the sum is rounded to the rows' type, as it is stored, and the norm is of the stored value
             if (p.r) add_rows(x[q], r[q]);
-            if (p.h)
+            if (p.h) {
                 store16<T, kVec>(row_at(static_cast<T*>(p.h), m, even, p.L, p.h_nb1, p.h_nb2), c0 + q * kChunk, lane, K, p.align,
                                  x[q]);
+                __syncwarp();  // encode_again may read a column that another lane has written
+            }
             widen(x[q], v[q]);
 #pragma unroll
             for (int j = 0; j < kPer; j += 2) {
@@ -434,20 +497,20 @@ __global__ void __launch_bounds__(kMaxThreads, std::max(1, norm_threads<T>() / k
             }
         }
         if (kAhead && m + step < rows) fetch(m + step, x, r);
-        float sum, other;
-        f2_unpack(sums, sum, other);
-        sum += other;
-#pragma unroll
-        for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(kAll, sum, s);
+        float lo, hi;
+        f2_unpack(sums, lo, hi);
+        double sum = warp_sum(lo + hi);
         if (!kWarpRows && warps > 1) {
             // two buffers in turn: a warp may be one row ahead of another's reads, not two
             if (lane == 0) part[turn][warp] = sum;
             __syncthreads();
-            sum = lane < warps ? part[turn][lane] : 0.0f;
+            const int w = lane & ((1 << (32 - __clz(warps - 1))) - 1);  // the warps' sums, over and over along the lanes
+            sum = w < warps ? part[turn][w] : 0.0;
 #pragma unroll
-            for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(kAll, sum, s);
+            for (int s = 16; s; s >>= 1)
+                if (s < warps) sum += __shfl_xor_sync(kAll, sum, s);
         }
-        const float inv = rsqrtf(fmaf(sum, p.inv_cols, p.eps));
+        const float inv = rsqrtf(fmaf((float)sum, p.inv_cols, p.eps));
 #pragma unroll
         for (int q = 0; q < kChunks; ++q) {
             if (!kAhead && p.gain) {
@@ -460,7 +523,11 @@ __global__ void __launch_bounds__(kMaxThreads, std::max(1, norm_threads<T>() / k
 #pragma unroll
             for (int j = 0; j < kPer; j += 2)
                 f2_unpack(mul_f32x2(f2_pack(v[q][j], v[q][j + 1]), f2_pack(g[q][j], g[q][j + 1])), v[q][j], v[q][j + 1]);
-            if (c0 + q * kChunk < K) encode16<kVec>(v[q], p.out, m, c0 + q * kChunk, lane);
+            if (c0 + q * kChunk < K) {
+                uint32_t word;
+                const uint32_t near = encode16<kVec, true>(v[q], p.out, m, c0 + q * kChunk, lane, word);
+                if (near) encode_again<T, kVec>(p, m, c0 + q * kChunk, lane, near, word, sum);
+            }
         }
     }
 }
@@ -484,7 +551,8 @@ __global__ void __launch_bounds__(kUnitThreads) quant8_kernel(const Quant8Params
     settle<T, kVec>(a, lane);
     float v[kPer];
     widen(a, v);
-    encode16<kVec>(v, p.out, row, chunk * kChunk, lane);
+    uint32_t word;
+    encode16<kVec, false>(v, p.out, row, chunk * kChunk, lane, word);
 }
 
 // Weight rows of 32-element ggml blocks (q8_0: f16 scale d and 32 int8; q4_0: f16 scale d and 16 bytes, element j in the
