@@ -258,6 +258,7 @@ kd_attn_status kd_attn_dequantize_fp8(kd_attn_ctx* ctx, const kd_fp8_rows* x, kd
  * x : [K, L, N] f32, f16 or bf16, any strides with dim 0 contiguous, K at most 32768
  * residual : as x (same type and sizes) or NULL
  * gain : device f32 [K], or NULL for unit gain;  eps >= 0
+ * The squares are summed in f32 (they overflow from |s| of about 1e19).
  * h : as x, or NULL: receives s, rounded to its type; the norm is taken of the rounded s whether or not h is
  *     given.  h may be x or residual itself. */
 kd_attn_status kd_attn_rms_norm_fp8(kd_attn_ctx* ctx, const kd_tensor* x, const kd_tensor* residual,

@@ -8,6 +8,8 @@
 //   kd::ops::attention            src/core/ops.hpp:107-207  (ops::attention, flash branch)
 //   kd::ops::linear               src/core/ops.hpp:27-42    (ops::linear: mul_mat + bias)
 //   kd::Linear                    src/core/module.hpp:87-110 (Linear's weight and bias)
+//   kd::Fp8Rows, kd::ops::rms_norm_fp8 / quantize_fp8 / dequantize_fp8 / linear_fp8
+//                                 RMSNorm and Linear on 8-bit operands (no counterpart in the reference)
 //   kd::dit_self_attention_block  src/models/crossdit.hpp:117-154 (DiTSelfAttention::forward whole:
 //                                 to_query/to_key/to_value, norms, RoPE, attention, out_layer)
 //   kd::dit_cross_attention_block src/models/crossdit.hpp:174-200 (DiTCrossAttention::forward whole)
@@ -116,6 +118,32 @@ struct Linear {
     }
 };
 
+// Rows of e4m3 codes with a power-of-two scale per 128 columns (kd_fp8_rows, whose layout kd_attn.h gives) in buffers
+// of the caller: codes of rows * pitch bytes, scales of scale_bytes(columns, rows), both 16-byte aligned.
+struct Fp8Rows {
+    void* codes = nullptr;
+    void* scales = nullptr;
+    int64_t columns = 0, rows = 0;
+    size_t pitch = 0;  // bytes between rows of codes: a multiple of 16 from `columns` on
+
+    // A pitch that suits the product best (whole blocks of 128).
+    static size_t suggested_pitch(int64_t columns) { return (size_t)((columns + 127) / 128 * 128); }
+    // 0 when the sizes are not supported.
+    static size_t scale_bytes(int64_t columns, int64_t rows) {
+        size_t n = 0;
+        return kd_attn_fp8_scale_bytes(columns, rows, &n) == KD_ATTN_OK ? n : 0;
+    }
+    kd_fp8_rows view() const {
+        kd_fp8_rows r{};
+        r.codes = codes;
+        r.scales = scales;
+        r.ne[0] = columns;
+        r.ne[1] = rows;
+        r.nb1 = pitch;
+        return r;
+    }
+};
+
 // Owns one kd_attn_ctx (per device).  Move-only.
 class Context {
 public:
@@ -174,6 +202,53 @@ inline bool linear(Context& ctx, const Tensor& x, const Linear& w, Tensor& y, vo
     const kd_linear tw = w.view();
     kd_tensor ty = y.view();
     return kd_attn_linear(ctx.get(), &tx, &tw, &ty, stream) == KD_ATTN_OK;
+}
+
+// x [K, L, N] (f32, f16 or bf16) into 8-bit rows (token l of sequence n is row n * L + l).
+inline bool quantize_fp8(Context& ctx, const Tensor& x, const Fp8Rows& out, void* stream = nullptr) {
+    if (!ctx.ok()) return false;
+    const kd_tensor tx = x.view();
+    kd_fp8_rows o = out.view();
+    return kd_attn_quantize_fp8(ctx.get(), &tx, &o, stream) == KD_ATTN_OK;
+}
+
+// A Linear's weight into 8-bit rows, laid out once for linear_fp8 (its bias is passed there).
+inline bool quantize_fp8(Context& ctx, const Linear& w, const Fp8Rows& out, void* stream = nullptr) {
+    if (!ctx.ok()) return false;
+    const kd_linear tw = w.view();
+    kd_fp8_rows o = out.view();
+    return kd_attn_quantize_weight_fp8(ctx.get(), &tw, &o, stream) == KD_ATTN_OK;
+}
+
+// 8-bit rows back into y [K, L, N].
+inline bool dequantize_fp8(Context& ctx, const Fp8Rows& x, Tensor& y, void* stream = nullptr) {
+    if (!ctx.ok()) return false;
+    const kd_fp8_rows tx = x.view();
+    kd_tensor ty = y.view();
+    return kd_attn_dequantize_fp8(ctx.get(), &tx, &ty, stream) == KD_ATTN_OK;
+}
+
+// RMSNorm::forward (module.hpp:163-180) of x + residual (nullptr: of x) over whole rows of K, into 8-bit rows; the sum
+// goes to h when given (which may be x or residual); gain: device f32 [K] or nullptr.
+inline bool rms_norm_fp8(Context& ctx, const Tensor& x, const Tensor* residual, const float* gain, float eps, Tensor* h,
+                         const Fp8Rows& out, void* stream = nullptr) {
+    if (!ctx.ok()) return false;
+    const kd_tensor tx = x.view();
+    kd_tensor tr{}, th{};
+    if (residual) tr = residual->view();
+    if (h) th = h->view();
+    kd_fp8_rows o = out.view();
+    return kd_attn_rms_norm_fp8(ctx.get(), &tx, residual ? &tr : nullptr, gain, eps, h ? &th : nullptr, &o, stream) ==
+           KD_ATTN_OK;
+}
+
+// linear on 8-bit operands: y [out, L, N] = x W^T + bias (device f32 [out] or nullptr).
+inline bool linear_fp8(Context& ctx, const Fp8Rows& x, const Fp8Rows& w, const float* bias, Tensor& y,
+                       void* stream = nullptr) {
+    if (!ctx.ok()) return false;
+    const kd_fp8_rows tx = x.view(), tw = w.view();
+    kd_tensor ty = y.view();
+    return kd_attn_linear_fp8(ctx.get(), &tx, &tw, bias, &ty, stream) == KD_ATTN_OK;
 }
 
 }  // namespace ops

@@ -70,3 +70,30 @@ def test_reference_restatement_agrees_with_torch():
     want = torch.from_numpy(v).float().to(torch.float8_e4m3fn).view(torch.uint8).numpy()
     got = fp8_ref.round_e4m3(v.astype(np.float32).astype(np.float64))
     assert np.array_equal(fp8_ref.VALUES[got], fp8_ref.VALUES[want])
+
+
+def build_host_test(kd, tmp_path):
+    """g++ -> tests/native/host_fp8_test linked against libkd_attn.so and cudart."""
+    gxx, cuda = shutil.which("g++"), os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    if gxx is None:
+        pytest.skip("g++ not available")
+    exe = str(tmp_path / "host_fp8_test")
+    lib_dir, rt = os.path.dirname(kd.LIB_PATH), os.path.join(cuda, "lib64")
+    cmd = [gxx, "-std=c++17", "-O2", "-Wall", "-Wextra", "-I", os.path.join(ROOT, "include"),
+           "-I", os.path.join(ROOT, "kandinsky.cpp_b200", "host"), "-I", os.path.join(cuda, "include"),
+           os.path.join(ROOT, "tests", "native", "host_fp8_test.cpp"), "-o", exe, kd.LIB_PATH, "-L", rt, "-lcudart",
+           f"-Wl,-rpath,{lib_dir}", f"-Wl,-rpath,{rt}"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-4000:]
+    return exe
+
+
+def test_host_layer_on_cpu(kd, tmp_path):
+    out = subprocess.run([build_host_test(kd, tmp_path), "--cpu"], capture_output=True, text=True, timeout=120)
+    assert out.returncode == 0 and out.stdout.strip() == "OK", out.stdout + out.stderr
+
+
+@pytest.mark.gpu
+def test_host_layer_on_gpu(kd, tmp_path):
+    out = subprocess.run([build_host_test(kd, tmp_path)], capture_output=True, text=True, timeout=120)
+    assert out.returncode == 0 and out.stdout.strip().endswith("OK"), out.stdout + out.stderr
