@@ -312,8 +312,10 @@ __device__ __forceinline__ void block_tops(float (&v)[kPer], uint32_t (&top)[4])
 }
 
 // A value within kNear steps of f32 of the middle between two (normal) codes, where its last bits decide, gives at most
-// kMiddle: the 20 fraction bits that a code drops, around one half, shifted up by 12.
-constexpr uint32_t kNear = 12, kMiddle = 2 * kNear << 12;
+// kMiddle: the 20 fraction bits that a code drops, around one half, shifted up by 12.  Four steps of 2^-24 (where a
+// significand is near 2): the norm's values carry the roundings of 1 / sqrt and of two products, half a step each, and
+// half of the mean's error; a wider window finds no more.
+constexpr uint32_t kNear = 4, kMiddle = 2 * kNear << 12;
 __device__ __forceinline__ uint32_t middle(float v) { return (__float_as_uint(v) << 12) + ((kNear - 0x80000u) << 12); }
 
 // 512 columns of a row from c0, sixteen values to a lane (zeros past K), into codes and scale bytes.  All lanes take
@@ -394,46 +396,64 @@ __device__ __forceinline__ P* row_at(P* base, long long m, bool even, long long 
 template <typename T>
 constexpr int norm_threads() { return sizeof(T) == 2 ? 768 : 512; }
 
-// The sum over a warp of values >= 0, to 2^-26 of the largest: in whole numbers, which one instruction adds exactly
-// (in f32 the five rounded steps would be off by as much as a value's own rounding, and move every value of the row
-// across the middles between codes).  NaN if any is, infinite if any is.
-__device__ __forceinline__ double warp_sum(float v) {
+// The sum over a warp of values >= 0 as total * 2^exponent, to 2^-26 of the largest: in whole numbers, which one
+// instruction adds exactly (in f32 the five rounded steps would be off by as much as a value's own rounding, and move
+// every value of the row across the middles between codes).  Not finite: an exponent of 1024 + 128, the largest in total.
+struct WarpSum {
+    uint32_t total;
+    int exponent;
+    __device__ float value() const {
+        if (exponent > 1024) return __uint_as_float(total);
+        const int half = exponent >> 1;  // (two factors: one may not be a normal number)
+        return (float)total * __uint_as_float((uint32_t)(half + 127) << 23) * __uint_as_float((uint32_t)(exponent - half + 127) << 23);
+    }
+    __device__ double exact() const {
+        if (exponent > 1024) return __uint_as_float(total);
+        return (double)total * __hiloint2double((exponent + 1023) << 20, 0);
+    }
+};
+__device__ __forceinline__ WarpSum warp_sum(float v) {
     const uint32_t top = __reduce_max_sync(kAll, __float_as_uint(v) & 0x7FFFFFFFu);
-    if (top >= kInfBits) return __uint_as_float(top);
-    const float lift = top < (64u << 23) ? 0x1p64f : 1.0f;             // so that the factor below is a normal number
+    if (top >= kInfBits) return WarpSum{top, 1024 + 128};
+    const bool low = top < 64u << 23;  // lifted, so that the factor below is a normal number
+    const float lift = low ? 0x1p64f : 1.0f;
     const uint32_t e = __float_as_uint(__uint_as_float(top) * lift) >> 23;  // lifted values are below 2^(e - 126)
-    const float unit = __uint_as_float((279u - e) << 23);              // 2^(152 - e): below 2^26
-    const uint32_t total = __reduce_add_sync(kAll, __float2uint_rn(v * lift * unit));
-    return (double)total * (1.0 / lift) * __hiloint2double((int)((e + (1023u - 152u)) << 20), 0);
+    const float unit = __uint_as_float((279u - e) << 23);                   // 2^(152 - e): below 2^26
+    return WarpSum{__reduce_add_sync(kAll, __float2uint_rn(v * lift * unit)), (int)e - 152 - (low ? 64 : 0)};
 }
 
-// The codes of some of a lane's values (bit j of `near`) once more, from the row in memory and in 64 bits: the value in
-// units of its scale, truncated to f32 with the last bit set if anything was dropped, which rounds as the value does.
+// 1 / sqrt(mean) within about half a step: CUDA's approximation and one Newton step.
+__device__ __forceinline__ float inverse_root(float mean) {
+    const float y = rsqrtf(mean);
+    const float more = fmaf(0.5f * y, fmaf(-mean * y, y, 1.0f), y);
+    return mean < __uint_as_float(kInfBits) ? more : y;
+}
+
+// The codes of some of a lane's values (bit j of `near`) once more, from h, the gain and the row's squares: |v| is above
+// the middle M between its neighbours if (h g f)^2 K > M^2 (squares + K eps), f being one over the block's scale, to some
+// 2^-50 in 64 bits.  One value in 115,000 comes here, which brings the codes that are not the exact value's from 5.4e-7
+// to 1e-7 of all (elementary f32 operations: 5.9e-7).  It costs the f32 norm of 31,744 x 1,792 89 -> 100 us with its
+// read-back and the bf16 norm of 4,096 columns 196 -> 201 us: the first visits on an SM fetch instructions that the
+// rows streaming through L2 have pushed out (a visit that does nothing but store a byte takes 93 us).
 template <typename T, bool kVec>
 __device__ __forceinline__ void encode_again(const Norm8Params& p, long long m, int c0, int lane, uint32_t near, uint32_t word,
-                                             double squares) {
-    const bool even = p.L >= p.out.rows;
-    const double inv = 1.0 / sqrt(squares / p.out.K + p.eps);
+                                             const Raw<T>& rows, const float (&gain)[kPer], float inv, double squares) {
+    const double right = fma((double)p.out.K, (double)p.eps, squares);
     for (; near; near &= near - 1) {
         const int j = __ffs(near) - 1, c = column<kVec>(c0, lane, j);
         if (c >= p.out.K) break;
-        float h;
-        if (p.h) {
-            h = to_f32(row_at(static_cast<const T*>(p.h), m, even, p.L, p.h_nb1, p.h_nb2)[c]);
-        } else {
-            T a = row_at(static_cast<const T*>(p.x), m, even, p.L, p.x_nb1, p.x_nb2)[c];
-            if (p.r) {
-                const T b = row_at(static_cast<const T*>(p.r), m, even, p.L, p.r_nb1, p.r_nb2)[c];
-                if constexpr (sizeof(T) == 4) a = __fadd_rn(a, b);
-                else a = __hadd(a, b);
-            }
-            h = to_f32(a);
-        }
-        const uint32_t byte = word >> (8 * (kVec ? lane >> 3 : j >> 2)) & 255u;
-        const double v = h * inv * (p.gain ? p.gain[c] : 1.0f) * fp8_scale_inverse(byte);
-        float f = __double2float_rz(v);
-        if ((double)f != v) f = __uint_as_float(__float_as_uint(f) | 1u);
-        p.out.codes[m * p.out.row_bytes + c] = (uint8_t)fp8_pack4(f, 0.0f, 0.0f, 0.0f);
+        float h = 0.0f, g = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            if (i == j) h = to_f32(get(rows, i)), g = gain[i];
+        const float f = fp8_scale_inverse(word >> (8 * (kVec ? lane >> 3 : j >> 2)) & 255u);
+        const uint32_t about = __float_as_uint(h * inv * g * f);
+        const uint32_t middle = (about & 0xFFF00000u) | 0x80000u;
+        const double a = (double)h * g * f, b = __uint_as_float(middle);
+        const double left = a * a * p.out.K, bar = b * b * right;
+        // one step of f32 to the side of the value (magnitudes: the sign is the top bit)
+        const uint32_t bits = left > bar ? middle + 1 : (left < bar ? middle - 1 : middle);
+        p.out.codes[m * p.out.row_bytes + c] = (uint8_t)fp8_pack4(__uint_as_float(bits), 0.0f, 0.0f, 0.0f);
     }
 }
 
@@ -444,7 +464,7 @@ template <typename T, bool kVec, int kMaxThreads, bool kWarpRows>
 __global__ void __launch_bounds__(kMaxThreads, std::max(1, norm_threads<T>() / kMaxThreads)) norm8_kernel(const __grid_constant__ Norm8Params p) {
     constexpr int kChunks = kMaxThreads > 512 ? 2 : 1;
     constexpr bool kAhead = kChunks == 1;  // a second row of 32 columns a thread does not fit the registers
-    __shared__ double part[2][32];
+    __shared__ WarpSum part[2][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int K = p.out.K;
     launch_next();
@@ -477,6 +497,7 @@ __global__ void __launch_bounds__(kMaxThreads, std::max(1, norm_threads<T>() / k
     for (long long m = first; m < rows; m += step, turn ^= 1) {
         if (!kAhead) fetch(m, x, r);
         float v[kChunks][kPer];
+        Raw<T> s[kChunks];
         uint64_t sums = f2_pack(0.0f, 0.0f);
 #pragma unroll
         for (int q = 0; q < kChunks; ++q) {
@@ -484,11 +505,10 @@ __global__ void __launch_bounds__(kMaxThreads, std::max(1, norm_threads<T>() / k
             if (p.r) settle<T, kVec>(r[q], lane);
             // the sum is rounded to the rows' type, as it is stored, and the norm is of the stored value
             if (p.r) add_rows(x[q], r[q]);
-            if (p.h) {
+            if (p.h)
                 store16<T, kVec>(row_at(static_cast<T*>(p.h), m, even, p.L, p.h_nb1, p.h_nb2), c0 + q * kChunk, lane, K, p.align,
                                  x[q]);
-                __syncwarp();  // encode_again may read a column that another lane has written
-            }
+            s[q] = x[q];
             widen(x[q], v[q]);
 #pragma unroll
             for (int j = 0; j < kPer; j += 2) {
@@ -499,18 +519,19 @@ __global__ void __launch_bounds__(kMaxThreads, std::max(1, norm_threads<T>() / k
         if (kAhead && m + step < rows) fetch(m + step, x, r);
         float lo, hi;
         f2_unpack(sums, lo, hi);
-        double sum = warp_sum(lo + hi);
+        const WarpSum mine = warp_sum(lo + hi);
+        float sum = mine.value();
         if (!kWarpRows && warps > 1) {
             // two buffers in turn: a warp may be one row ahead of another's reads, not two
-            if (lane == 0) part[turn][warp] = sum;
+            if (lane == 0) part[turn][warp] = mine;
             __syncthreads();
             const int w = lane & ((1 << (32 - __clz(warps - 1))) - 1);  // the warps' sums, over and over along the lanes
-            sum = w < warps ? part[turn][w] : 0.0;
+            sum = w < warps ? part[turn][w].value() : 0.0f;
 #pragma unroll
             for (int s = 16; s; s >>= 1)
                 if (s < warps) sum += __shfl_xor_sync(kAll, sum, s);
         }
-        const float inv = rsqrtf(fmaf((float)sum, p.inv_cols, p.eps));
+        const float inv = inverse_root(fmaf(sum, p.inv_cols, p.eps));
 #pragma unroll
         for (int q = 0; q < kChunks; ++q) {
             if (!kAhead && p.gain) {
@@ -526,7 +547,14 @@ __global__ void __launch_bounds__(kMaxThreads, std::max(1, norm_threads<T>() / k
             if (c0 + q * kChunk < K) {
                 uint32_t word;
                 const uint32_t near = encode16<kVec, true>(v[q], p.out, m, c0 + q * kChunk, lane, word);
-                if (near) encode_again<T, kVec>(p, m, c0 + q * kChunk, lane, near, word, sum);
+                if (near) {
+                    double squares = mine.exact();
+                    if (!kWarpRows && warps > 1) {
+                        squares = 0.0;
+                        for (int w = 0; w < warps; ++w) squares += part[turn][w].exact();
+                    }
+                    encode_again<T, kVec>(p, m, c0 + q * kChunk, lane, near, word, s[q], g[q], inv, squares);
+                }
             }
         }
     }
