@@ -162,6 +162,7 @@ class Fp8Rows:
         if codes.device != scales.device:
             raise ValueError("codes and scales must be on one device")
         self.codes, self.scales, self.rows, self.in_features = codes, scales, rows, K
+        self.device = codes.get_device()  # -1: not on a GPU
         self.struct = _Fp8RowsStruct.from_buffer_copy(_FP8_ROWS.pack(codes.data_ptr(), scales.data_ptr(), K, rows, pitch[0]))
 
     @staticmethod
@@ -341,15 +342,16 @@ def nccl_unique_id() -> bytes:
 _RAW_STREAM = []
 
 
-def _stream_ptr(stream):
+def _stream_ptr(stream, device=None):
+    """A stream's handle; None: the current stream of `device`, or of the current device."""
     if stream is None:
         import torch
         if _RAW_STREAM:  # the current stream's handle without an object around it
-            return ctypes.c_void_p(_RAW_STREAM[0](torch.cuda.current_device()))
+            return ctypes.c_void_p(_RAW_STREAM[0](torch.cuda.current_device() if device is None else device))
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         if raw is not None and torch.cuda.is_initialized():
             _RAW_STREAM.append(raw)
-        stream = torch.cuda.current_stream()
+        stream = torch.cuda.current_stream(device)
     return ctypes.c_void_p(stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream))
 
 
@@ -466,34 +468,60 @@ class Context:
         self.check(lib.kd_attn_linear(self.handle, _ref(x), ctypes.byref(w), _ref(y), _stream_ptr(stream)))
         return y
 
+    def _here(self, *tensors):
+        """Refuses tensors (or 8-bit rows) that are not on this context's device: the kernels would read elsewhere."""
+        for t in tensors:
+            if t is not None and (t.device if isinstance(t, Fp8Rows) else t.get_device()) != self.device:
+                raise ValueError(f"a tensor is not on cuda:{self.device}")
+
+    def _vector(self, t, n, name):
+        """The address of an f32 vector of n contiguous elements on this context's device, or None."""
+        if t is None:
+            return None
+        if t.dtype not in _TORCH_TYPES:
+            _torch_type(t.dtype)
+        if _TORCH_TYPES[t.dtype][0] != F32 or t.numel() != n or not t.is_contiguous():
+            raise ValueError(f"{name} must be {n} contiguous f32 values")
+        self._here(t)
+        return ctypes.c_void_p(t.data_ptr())
+
     def quantize_fp8(self, x, out, stream=None):
         """x (N, L, K), (L, K) or (K,) f32/f16/bf16 into the 8-bit rows out (an Fp8Rows of N * L rows)."""
-        self.check(lib.kd_attn_quantize_fp8(self.handle, _ref(x), ctypes.byref(out.struct), _stream_ptr(stream)))
+        self._here(x, out)
+        self.check(lib.kd_attn_quantize_fp8(self.handle, _ref(x), ctypes.byref(out.struct),
+                                            _stream_ptr(stream, self.device)))
         return out
 
     def quantize_weight_fp8(self, w, out, stream=None):
         """The weight of a KdLinear into 8-bit rows, laid out once for ``linear_fp8``; its bias is not read."""
+        self._here(out)
         self.check(lib.kd_attn_quantize_weight_fp8(self.handle, ctypes.byref(w), ctypes.byref(out.struct),
-                                                   _stream_ptr(stream)))
+                                                   _stream_ptr(stream, self.device)))
         return out
 
     def dequantize_fp8(self, x, y, stream=None):
         """The values of the 8-bit rows x into y (N, L, K) f32/f16/bf16."""
-        self.check(lib.kd_attn_dequantize_fp8(self.handle, ctypes.byref(x.struct), _ref(y), _stream_ptr(stream)))
+        self._here(x, y)
+        self.check(lib.kd_attn_dequantize_fp8(self.handle, ctypes.byref(x.struct), _ref(y),
+                                              _stream_ptr(stream, self.device)))
         return y
 
     def rms_norm_fp8(self, x, out, residual=None, gain=None, eps=1e-6, h=None, stream=None):
         """s = x + residual (rounded to x's type, into h when given), out = s / sqrt(mean(s^2) + eps) * gain in 8
         bits.  x, residual, h (N, L, K) of one type f32/f16/bf16; gain f32 (K,) or None; h may be x or residual."""
-        self.check(lib.kd_attn_rms_norm_fp8(self.handle, _ref(x), _ref(residual), _ptr(gain), float(eps), _ref(h),
-                                            ctypes.byref(out.struct), _stream_ptr(stream)))
+        self._here(x, residual, h, out)
+        self.check(lib.kd_attn_rms_norm_fp8(self.handle, _ref(x), _ref(residual),
+                                            self._vector(gain, out.in_features, "gain"), float(eps), _ref(h),
+                                            ctypes.byref(out.struct), _stream_ptr(stream, self.device)))
         return out
 
     def linear_fp8(self, x, w, y, bias=None, stream=None):
         """ops::linear on 8-bit operands: y (N, L, C) f32/bf16/f16 = x W^T + b; x an Fp8Rows of N * L rows, w an
         Fp8Rows of C rows, bias f32 (C,) or None."""
-        self.check(lib.kd_attn_linear_fp8(self.handle, ctypes.byref(x.struct), ctypes.byref(w.struct), _ptr(bias),
-                                          _ref(y), _stream_ptr(stream)))
+        self._here(x, w, y)
+        self.check(lib.kd_attn_linear_fp8(self.handle, ctypes.byref(x.struct), ctypes.byref(w.struct),
+                                          self._vector(bias, w.rows, "bias"), _ref(y),
+                                          _stream_ptr(stream, self.device)))
         return y
 
     def self_attention_block(self, x, wq, wk, wv, wo, n_head, y, q_gain=None, k_gain=None, eps=1e-6, rope=None,

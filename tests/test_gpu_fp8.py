@@ -482,5 +482,16 @@ def test_refusals(ctx, kd):
     refused(lambda: ctx.linear_fp8(pitch, w, z(4, 32)), bad)
     off = kd.Fp8Rows(z(4 * 80 + 8, dtype=torch.uint8)[8:].view(4, 80), r.scales, 64)  # codes at 8 bytes
     refused(lambda: ctx.linear_fp8(off, w, z(4, 32)), bad)
+    for call in (lambda: ctx.quantize_fp8(torch.zeros(4, 64), r),                    # host memory
+                 lambda: ctx.linear_fp8(kd.Fp8Rows.empty(4, 64, device="cpu"), w, z(4, 32)),
+                 lambda: ctx.linear_fp8(r, w, torch.zeros(4, 32)),
+                 lambda: ctx.linear_fp8(r, w, z(4, 32), bias=torch.zeros(32)),
+                 lambda: ctx.linear_fp8(r, w, z(4, 32), bias=z(31)),
+                 lambda: ctx.linear_fp8(r, w, z(4, 32), bias=z(32, dtype=torch.bfloat16)),
+                 lambda: ctx.rms_norm_fp8(z(4, 64), r, gain=z(128)[::2]),
+                 lambda: ctx.rms_norm_fp8(z(4, 64), r, h=torch.zeros(4, 64)),
+                 lambda: ctx.dequantize_fp8(r, torch.zeros(4, 64))):
+        with pytest.raises(ValueError):
+            call()
     ctx.linear_fp8(r, w, z(4, 32))                                                   # the context stays usable
     ctx.device_status()
