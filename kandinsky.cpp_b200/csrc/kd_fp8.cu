@@ -391,8 +391,8 @@ __device__ __forceinline__ P* row_at(P* base, long long m, bool even, long long 
 }
 
 // Threads of the norm that an SM is to hold: 768 (80 registers) for 16-bit rows, whose loads in flight are small, 512
-// (128 registers) for f32.  Measured at 31,744 x 4,096 bf16 with residual: 512 threads 176 us, 768 154 us, 1,024 170 us
-// (spills).
+// (128 registers) for f32.  31,744 x 4,096 bf16 with residual, before its arithmetic was packed (136 us since): 512
+// threads 176 us, 768 154 us, 1,024 170 us (spills).
 template <typename T>
 constexpr int norm_threads() { return sizeof(T) == 2 ? 768 : 512; }
 
