@@ -588,7 +588,8 @@ __global__ void __launch_bounds__(kUnitThreads) quant8_kernel(const Quant8Params
 // Blocks are 34 or 18 bytes long, so a lane reads 16-bit words.  (Bringing the warp's bytes into shared memory in
 // 16-byte loads first was slower, 13.6 us against 11.0 for 4,096 x 4,096 q8_0: instructions bound it.)  So the codes q
 // become f32 by their place in a significand, the largest is found among them, and d and the new scale, a power of
-// two, are multiplied once: d * q * 2^-e is exact whichever comes first (11 and 8 significant bits).
+// two, are multiplied once: d * q * 2^-e is exact whichever comes first (11 and 8 significant bits).  Only where the largest
+// code is not 0, which bounds |d| by the new scale; a ggml block of zeros under any finite d takes the factor 0.
 constexpr int kGgmlWarps = 4;
 template <bool kQ4>
 __global__ void __launch_bounds__(32 * kGgmlWarps) quant8_ggml_kernel(const uint8_t* w, long long row_bytes, const Fp8Rows o) {
@@ -633,7 +634,7 @@ __global__ void __launch_bounds__(32 * kGgmlWarps) quant8_ggml_kernel(const uint
     for (int s = 2; s; s >>= 1) top = max(top, __shfl_xor_sync(kAll, top, s));
     const uint32_t byte = fp8_scale_byte(top);
     if (!live) return;
-    d = nan ? __uint_as_float(0x7FFFFFFFu) : d * fp8_scale_inverse(byte);
+    d = nan ? __uint_as_float(0x7FFFFFFFu) : (most == 0.0f ? 0.0f : d * fp8_scale_inverse(byte));
     uint4* dst = reinterpret_cast<uint4*>(o.codes + row * o.row_bytes + c);
     const uint64_t dd = f2_pack(d, d);
 #pragma unroll
