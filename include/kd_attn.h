@@ -225,7 +225,7 @@ kd_attn_status kd_attn_linear(kd_attn_ctx* ctx, const kd_tensor* x, const kd_lin
  * scales: for each row and block b of 128 columns a byte s, the block's scale being 2^(s - 127); the byte of
  * (r, b) is at ((r / 128) * T + b / 4) * 512 + (r % 32) * 16 + (r % 128 / 32) * 4 + b % 4 with
  * T = ceil(ceil(K / 128) / 4) (kd_attn_fp8_scale_bytes in all, 16-byte aligned): the order in which the
- * tensor core takes them.  An element is worth code * 2^(s - 127).
+ * tensor core takes them.  An element is worth code * 2^(s - 127), and NaN under s = 255.
  *
  * The writers choose the smallest scale >= 2^-126 with max|v| <= 448 * scale over the block and round codes to
  * nearest even.  A NaN or an infinity becomes the NaN code and does not count for the scale.  Rows and columns

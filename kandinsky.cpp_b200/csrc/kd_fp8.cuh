@@ -26,7 +26,12 @@ __device__ __forceinline__ uint32_t fp8_scale_byte(uint32_t amax) {
     const int b = (int)((amax + 0x1FFFFFu) >> 23) - 8;
     return (uint32_t)max(b, 1);
 }
-__device__ __forceinline__ float fp8_scale_value(uint32_t byte) { return __uint_as_float(byte << 23); }
+// 2^(byte - 127), NaN for 255, as the tensor core takes them.  The writers make 1 .. 247; rows from elsewhere may hold 0
+// (2^-127, a subnormal) and 255, where the exponent field alone would say 0 and infinity.
+__device__ __forceinline__ float fp8_scale_value(uint32_t byte) {
+    return __uint_as_float(byte << 23 | (byte - 1u >= 254u ? 0x400000u : 0u));
+}
+// Of the writers' bytes.
 __device__ __forceinline__ float fp8_scale_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
 
 // Programmatic launches: a kernel of this path may start while the one before it in the stream runs out, and sets up

@@ -52,3 +52,53 @@ def test_ggml_zero_codes_under_any_scale(ctx, kd, name, K):
     assert np.array_equal(gs, s)
     assert np.array_equal(fp8_ref.VALUES[got], fp8_ref.VALUES[want], equal_nan=True)
     assert not np.isnan(fp8_ref.VALUES[got[:C - 2]]).any()
+
+
+def bytes_operand(kd, codes, scales):
+    """An Fp8Rows of given codes (R, K) and scale bytes (R, blocks)."""
+    R, K = codes.shape
+    r = kd.Fp8Rows.empty(R, K)
+    c = np.zeros((R, r.codes.shape[1]), np.uint8)
+    c[:, :K] = codes
+    t = np.zeros(r.scales.numel(), np.uint8)
+    t[fp8_ref.tile_offsets(R, K)] = scales
+    r.codes.view(torch.uint8).copy_(torch.from_numpy(c))
+    r.scales.copy_(torch.from_numpy(t))
+    return r
+
+
+def bytes_values(codes, scales):
+    """What such rows are worth in float64: code * 2^(byte - 127), and NaN under the byte 255."""
+    f = np.ldexp(1.0, scales.astype(int) - 127)
+    f[scales == 255] = np.nan
+    return fp8_ref.VALUES[codes] * np.repeat(f, 128, axis=1)[:, :codes.shape[1]]
+
+
+@pytest.mark.parametrize("pad", [0, 1])
+def test_read_back_of_every_scale_byte(ctx, kd, pad):
+    """All 256 codes under all 256 scale bytes, into aligned rows and into rows that start anywhere."""
+    codes = np.tile(np.arange(256, dtype=np.uint8), (256, 1))
+    scales = np.repeat(np.arange(256, dtype=np.uint8)[:, None], 2, axis=1)
+    r = bytes_operand(kd, codes, scales)
+    want = torch.from_numpy(bytes_values(codes, scales)).to(torch.float32)  # exact but for what is beyond f32
+    for dtype in TORCH.values():
+        y = torch.empty(256, 256 + pad, device="cuda", dtype=dtype)[:, pad:]
+        ctx.dequantize_fp8(r, y)
+        assert torch.equal(torch.nan_to_num(y.cpu().float(), nan=12345.0), torch.nan_to_num(want.to(dtype).float(), nan=12345.0))
+
+
+@pytest.mark.parametrize("M", [5, 300])
+def test_product_of_the_outermost_scale_bytes(ctx, kd, M):
+    """Scales of 2^-127 against 2^127 in either operand, and a block under the byte 255, which makes its row NaN."""
+    K, N = 256, 130
+    rng = np.random.default_rng(M)
+    cx, cw = (rng.integers(0, 126, (n, K)).astype(np.uint8) | (rng.integers(0, 2, (n, K)) << 7).astype(np.uint8) for n in (M, N))
+    for bx, bw in ((0, 254), (254, 0)):
+        sx, sw = np.full((M, 2), bx, np.uint8), np.full((N, 2), bw, np.uint8)
+        sx[3, 1] = 255
+        y = torch.empty(M, N, device="cuda")
+        ctx.linear_fp8(bytes_operand(kd, cx, sx), bytes_operand(kd, cw, sw), y)
+        assert torch.isnan(y[3]).all() and int(torch.isnan(y).any(1).sum()) == 1
+        keep = np.arange(M) != 3
+        check_product(y[torch.from_numpy(keep).cuda()], bytes_values(cx, sx)[keep], bytes_values(cw, sw), None, "f32", f"{bx} {bw}")
+    ctx.device_status()
