@@ -37,7 +37,8 @@ __device__ __forceinline__ float fp8_scale_inverse(uint32_t byte) { return __uin
 // Programmatic launches: a kernel of this path may start while the one before it in the stream runs out, and sets up
 // its barriers, tensor memory and registers meanwhile.  launch_next: the next one may start; called once this CTA holds
 // all that it will ever ask the SM for.  wait_for_previous: everything before in the stream has finished and is visible;
-// every thread calls it before it touches global memory.
+// every thread calls it before it touches global memory, and then loads by plain loads: read-only ones (__ldg) ask that
+// the data stay as they are for the kernel's whole time, of which the end of the kernel that writes them may be a part.
 __device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

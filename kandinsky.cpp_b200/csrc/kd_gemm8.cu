@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(kSThreads)
     } else {
         const int q = warp & 3, half = (warp - 2) >> 2;  // TMEM lanes 32 q .. of this warp, every other 16 columns
         const int f = q * 32 + lane, n = n0 + f;
-        const float bias = direct && p.bias && n < p.N ? __ldg(p.bias + n) : 0.0f;
+        const float bias = direct && p.bias && n < p.N ? p.bias[n] : 0.0f;
         const bool ok = __all_sync(0xffffffffu, mbar_wait(done, 0, ctl, kErrTimeoutO));
         tc_fence_after();
         if (ok && *reinterpret_cast<volatile unsigned*>(abort_flag) == 0) {
@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(kSThreads)
             const int n = n0 + lane * 4, step = p.splits * kSJoinWarps;
             float b[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) b[j] = p.bias && n + j < p.N ? __ldg(p.bias + n + j) : 0.0f;
+            for (int j = 0; j < 4; ++j) b[j] = p.bias && n + j < p.N ? p.bias[n + j] : 0.0f;
             for (int c0 = (int)rank + p.splits * (warp - 2); c0 < p.M; c0 += 2 * step) {
                 float4 a[2];
 #pragma unroll
@@ -677,7 +677,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
             {  // its bias, while the MMAs run
                 const int i = threadIdx.x - g * (32 * kPGroupWarps);
                 if (uses) named_bar_sync(1 + g, 32 * kPGroupWarps);
-                if (i < pn) bias[i] = p.bias && np + i < p.N ? __ldg(p.bias + np + i) : 0.0f;
+                if (i < pn) bias[i] = p.bias && np + i < p.N ? p.bias[np + i] : 0.0f;
                 named_bar_sync(1 + g, 32 * kPGroupWarps);
             }
             // After a wait gave up the group still goes through its tiles, without waiting again: its warps meet at the

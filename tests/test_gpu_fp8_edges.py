@@ -102,3 +102,32 @@ def test_product_of_the_outermost_scale_bytes(ctx, kd, M):
         keep = np.arange(M) != 3
         check_product(y[torch.from_numpy(keep).cuda()], bytes_values(cx, sx)[keep], bytes_values(cw, sw), None, "f32", f"{bx} {bw}")
     ctx.device_status()
+
+
+@pytest.mark.parametrize("M", [3, 100, 300])
+def test_vectors_written_by_the_call_before(ctx, kd, M):
+    """A bias that the product before wrote, and a gain likewise, in one buffer over and over: the bits that the same
+    calls give with a wait after each."""
+    K, C = 256, 640
+    w = operand(kd, hidden(C, K, 81) / np.sqrt(K))[0]
+    x, x64 = operand(kd, hidden(M, K, 82))
+    ones = [operand(kd, hidden(1, K, 83 + i))[0] for i in range(2)]
+    rows = dev(hidden(M, C, 85), "bf16")
+
+    def chain(sync):
+        v, out = torch.zeros(C, device="cuda"), []
+        for i in range(30):
+            y, r = torch.empty(M, C, device="cuda"), kd.Fp8Rows.empty(M, C)
+            for call in (lambda: ctx.linear_fp8(ones[i & 1], w, v), lambda: ctx.linear_fp8(x, w, y, bias=v),
+                         lambda: ctx.linear_fp8(ones[1 - (i & 1)], w, v), lambda: ctx.rms_norm_fp8(rows, r, gain=v)):
+                call()
+                if sync:
+                    torch.cuda.synchronize()
+            out += [y, r.codes.view(torch.uint8)[:, :C], r.scales.clone()]
+        torch.cuda.synchronize()
+        return out
+
+    fast, slow = chain(False), chain(True)
+    assert all(torch.equal(a, b) for a, b in zip(fast, slow))
+    assert not torch.equal(fast[0], fast[3])
+    ctx.device_status()
