@@ -230,6 +230,7 @@ kd_attn_status kd_attn_linear(kd_attn_ctx* ctx, const kd_tensor* x, const kd_lin
  * The writers choose the smallest scale >= 2^-126 with max|v| <= 448 * scale over the block and round codes to
  * nearest even.  A NaN or an infinity becomes the NaN code and does not count for the scale.  Rows and columns
  * outside the given sizes are left as they were, but for the up to 15 code bytes from K to the next multiple of 16.
+ * Rows of a tensor that is written may lie in any order and at any distance, but not over each other.
  * K is at most 2^20 and rows at most 2^24. */
 typedef struct {
     void* codes;    /* device */

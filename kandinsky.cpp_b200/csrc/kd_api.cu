@@ -16,6 +16,7 @@
 #include <vector>
 
 #include "../../include/kd_attn.h"
+#include "kd_host.h"
 #include "kd_internal.h"
 
 using namespace kd;
@@ -1315,7 +1316,7 @@ kd_attn_status check_token_rows(kd_attn_ctx* ctx, const kd_tensor* t, const char
     const size_t es = elt_size(t->type);
     if (reinterpret_cast<uintptr_t>(t->data) % es || nb[1] % es || nb[2] % es)
         return fail(ctx, KD_ATTN_ERR_UNSUPPORTED, "%s: address or strides are not whole elements", name);
-    if (written && ((t->ne[1] > 1 && nb[1] < es * (uint64_t)K) || (t->ne[2] > 1 && nb[2] < es * (uint64_t)K)))
+    if (written && rows_overlap(es * (uint64_t)K, nb[1], nb[2], t->ne[1], t->ne[2]))
         return fail(ctx, KD_ATTN_ERR_INVALID_ARGUMENT, "%s: its rows overlap", name);
     out->nb1 = (long long)nb[1];
     out->nb2 = (long long)nb[2];

@@ -131,3 +131,25 @@ def test_vectors_written_by_the_call_before(ctx, kd, M):
     assert all(torch.equal(a, b) for a, b in zip(fast, slow))
     assert not torch.equal(fast[0], fast[3])
     ctx.device_status()
+
+
+def test_written_rows_over_each_other_are_refused(ctx, kd):
+    """Tensors whose rows meet across tokens and sequences are refused as outputs; rows that interleave are written."""
+    K, flat = 64, lambda n: torch.full((n,), 9.0, device="cuda")
+    for N, L, sn, sl in ((3, 4, K, K), (3, 4, K, 2 * K), (2, 4, 4 * K, 2 * K), (2, 2, K, 2 * K - 1), (2, 3, 2 * K + 1, K)):
+        v, r, w = flat(4096).as_strided((N, L, K), (sn, sl, 1)), kd.Fp8Rows.empty(N * L, K), kd.Fp8Rows.empty(K, K)
+        x = torch.zeros(N, L, K, device="cuda")
+        for call in (lambda: ctx.dequantize_fp8(r, v), lambda: ctx.rms_norm_fp8(x, r, h=v), lambda: ctx.linear_fp8(r, w, v)):
+            with pytest.raises(kd.KdAttnError) as e:
+                call()
+            assert e.value.status == kd.ERR_INVALID_ARGUMENT and "overlap" in str(e.value)
+        assert ctx.quantize_fp8(v, r) is r  # (as an input they are rows like others)
+    for N, L, sn, sl in ((2, 4, K, 2 * K), (2, 4, 3 * K, 2 * K), (2, 2, 3 * K, 2 * K), (2, 2, K + 1, 2 * K + 2), (3, 2, K, 4 * K)):
+        x = dev(hidden(N * L, K, 95))
+        r = kd.Fp8Rows.empty(N * L, K)
+        ctx.quantize_fp8(x, r)
+        base = flat(4096)
+        v = base.as_strided((N, L, K), (sn, sl, 1))
+        ctx.dequantize_fp8(r, v)
+        assert np.array_equal(f64(v.reshape(N * L, K)), fp8_ref.decode(*rows_of(r)))
+        assert int((base != 9).sum()) <= N * L * K
