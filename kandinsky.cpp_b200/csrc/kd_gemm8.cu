@@ -8,9 +8,9 @@
 // scale id; the four instructions of a block name the same byte, and one 32-bit TMEM column holds the bytes of four
 // blocks (512 columns).
 #include <algorithm>
-#include <atomic>
 
 #include "kd_fp8.cuh"
+#include "kd_host.h"
 #include "kd_internal.h"
 
 namespace kd {
@@ -120,14 +120,9 @@ __device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) { retu
 
 // Allows a kernel its dynamic shared memory, once on each device.
 template <typename K>
-cudaError_t allow_smem(K kern, int bytes, std::atomic<unsigned long long>& done) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    const unsigned long long bit = 1ull << (dev & 63);
-    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_release);
+cudaError_t allow_smem(K kern, int bytes, int device, PerDevice& done) {
+    cudaError_t e = cudaSuccess;
+    done.get(device, [&] { return (e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) == cudaSuccess; });
     return e;
 }
 
@@ -793,27 +788,30 @@ __global__ void __launch_bounds__(kPThreads, 1)
 template <typename TO, int kParts, bool kWide>
 cudaError_t many_launch(const CUtensorMap* tm, const Gemm8Params& p, int num_sms, cudaStream_t st) {
     auto kern = gemm8_many_kernel<TO, kParts, kWide>;
-    static std::atomic<unsigned long long> ready{0};
-    cudaError_t e = allow_smem(kern, kPSmem, ready);
+    static PerDevice ready, pairs;
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess) e = allow_smem(kern, kPSmem, device, ready);
     if (e != cudaSuccess) return e;
     const long long tiles = (long long)((p.M + kPairM - 1) / kPairM) * ((p.N + p.nt * p.parts - 1) / (p.nt * p.parts));
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.blockDim = dim3(kPThreads);
-    cfg.dynamicSmemBytes = kPSmem;
-    cfg.stream = st;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    cfg.gridDim = dim3((unsigned)(2 * (num_sms / 2)));
-    // pairs that can be resident at one time; asked once, for every B200 is alike
-    static const int resident = [&] {
+    // pairs that can be resident at one time
+    const int resident = pairs.get(device, [&] {
+        cudaLaunchConfig_t cfg{};
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 2;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.gridDim = dim3((unsigned)(2 * (num_sms / 2)));
+        cfg.blockDim = dim3(kPThreads);
+        cfg.dynamicSmemBytes = kPSmem;
+        cfg.stream = st;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
         int n = 0;
-        return cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess ? n : 0;
-    }();
-    if (resident <= 0) return cudaErrorInvalidConfiguration;
+        e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
+        return e == cudaSuccess ? n : 0;
+    });
+    if (resident <= 0) return e != cudaSuccess ? e : cudaErrorInvalidConfiguration;
     return launch_following(kern, dim3((unsigned)(2 * (tiles < resident ? tiles : resident))), kPThreads, kPSmem, 2, st, tm[0],
                             tm[1], tm[2], tm[3], p);
 }
@@ -827,8 +825,10 @@ cudaError_t many_typed(const CUtensorMap* tm, const Gemm8Params& p, int num_sms,
 template <typename TO>
 cudaError_t few_typed(const CUtensorMap& tmX, const CUtensorMap& tmW, const Gemm8Params& p, cudaStream_t st) {
     auto kern = gemm8_few_kernel<TO>;
-    static std::atomic<unsigned long long> ready{0};
-    cudaError_t e = allow_smem(kern, 232448, ready);
+    static PerDevice ready;
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess) e = allow_smem(kern, 232448, device, ready);
     if (e != cudaSuccess) return e;
     return launch_following(kern, dim3((unsigned)((p.N + kGemm8BoxRows - 1) / kGemm8BoxRows) * (unsigned)p.splits), kSThreads,
                             few_smem(p.nt, ((p.K + 127) / 128 + p.splits - 1) / p.splits), (unsigned)p.splits, st, tmX, tmW, p);

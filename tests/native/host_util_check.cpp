@@ -33,8 +33,21 @@ static int check_rows_overlap() {
     return 0;
 }
 
+// PerDevice: failures are asked again, answers are kept, each for its own device; devices beyond the table are asked anew.
+static int check_per_device() {
+    kd::PerDevice v;
+    int asked = 0;
+    auto answer = [&](int n) { return [&asked, n] { return ++asked, n; }; };
+    const bool good = v.get(0, answer(0)) == 0 && v.get(0, answer(-3)) == -3 && v.get(0, answer(74)) == 74 && asked == 3 &&
+                      v.get(0, answer(5)) == 74 && asked == 3 && v.get(1, answer(66)) == 66 && v.get(0, answer(1)) == 74 &&
+                      v.get(1, answer(1)) == 66 && asked == 4 && v.get(64, answer(7)) == 7 && v.get(64, answer(8)) == 8 &&
+                      v.get(-1, answer(9)) == 9 && asked == 7;
+    if (!good) printf("PerDevice\n");
+    return good ? 0 : 1;
+}
+
 int main() {
-    const int bad = check_rows_overlap();
+    const int bad = check_rows_overlap() + check_per_device();
     if (!bad) printf("OK\n");
     return bad;
 }
