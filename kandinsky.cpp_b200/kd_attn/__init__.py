@@ -118,6 +118,7 @@ class KdLinear(ctypes.Structure):
     """kd_linear: a Linear layer's weight in ggml layout [K, C] (C rows of K elements of `type`) + f32 bias."""
     _fields_ = [("data", ctypes.c_void_p), ("type", ctypes.c_int32), ("ne", ctypes.c_int64 * 2),
                 ("nb1", ctypes.c_size_t), ("bias", ctypes.c_void_p)]
+    device = None  # index of the GPU that holds the weight (-1: not on a GPU) where `of` took it from a tensor
 
     @staticmethod
     def of(weight, type, in_features, out_features, bias=None):
@@ -130,6 +131,7 @@ class KdLinear(ctypes.Structure):
         w.ne[1] = int(out_features)
         w.nb1 = weight.stride(0) * weight.element_size()
         w.bias = None if bias is None else bias.data_ptr()
+        w.device = weight.get_device()
         return w
 
 
@@ -495,6 +497,8 @@ class Context:
     def quantize_weight_fp8(self, w, out, stream=None):
         """The weight of a KdLinear into 8-bit rows, laid out once for ``linear_fp8``; its bias is not read."""
         self._here(out)
+        if w.device not in (None, self.device):
+            raise ValueError(f"the weight is not on cuda:{self.device}")
         self.check(lib.kd_attn_quantize_weight_fp8(self.handle, ctypes.byref(w), ctypes.byref(out.struct),
                                                    _stream_ptr(stream, self.device)))
         return out

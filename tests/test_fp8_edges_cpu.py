@@ -5,6 +5,7 @@ import shutil
 import subprocess
 
 import pytest
+import torch
 
 from test_descriptors import ROOT
 
@@ -19,3 +20,17 @@ def test_host_helpers(tmp_path):
     assert r.returncode == 0, r.stderr[-3000:]
     out = subprocess.run([exe], capture_output=True, text=True, timeout=60)
     assert out.returncode == 0 and out.stdout.strip() == "OK", out.stdout + out.stderr
+
+
+def test_weight_elsewhere_is_refused(kd):
+    """A weight in host memory, or on another GPU than the context's, is turned away before the library is called."""
+    ctx = object.__new__(kd.Context)  # (no GPU here: what checks arguments needs only the device's index)
+    ctx.handle, ctx.device = None, 0
+    out = kd.Fp8Rows.empty(32, 64, device="cpu")
+    out.device = 0
+    w = kd.KdLinear.of(torch.zeros(32, 68, dtype=torch.uint8), kd.Q8_0, 64, 32)
+    assert w.device == -1 and kd.KdLinear().device is None
+    for device in (-1, 1):
+        w.device = device
+        with pytest.raises(ValueError):
+            ctx.quantize_weight_fp8(w, out)
