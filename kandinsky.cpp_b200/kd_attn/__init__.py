@@ -143,6 +143,12 @@ class _Fp8RowsStruct(ctypes.Structure):
 _FP8_ROWS = struct.Struct("@PP2qN")
 
 
+@functools.lru_cache(maxsize=None)
+def _code_types():
+    import torch
+    return torch.float8_e4m3fn, torch.uint8
+
+
 class Fp8Rows:
     """kd_fp8_rows: rows of e4m3 codes with a power-of-two scale per 128 columns, an operand of ``linear_fp8``.
 
@@ -152,8 +158,8 @@ class Fp8Rows:
 
     def __init__(self, codes, scales, in_features):
         shape, K = codes.shape, int(in_features)
-        if len(shape) != 2 or codes.element_size() != 1:
-            raise ValueError("codes must be a 2-D tensor of bytes")
+        if len(shape) != 2 or codes.dtype not in _code_types():
+            raise ValueError("codes must be a 2-D tensor of float8_e4m3fn or uint8")
         rows, pitch = shape[0], codes.stride()
         if pitch[1] != 1 and shape[1] > 1:
             raise ValueError("code rows must be contiguous")

@@ -34,3 +34,13 @@ def test_weight_elsewhere_is_refused(kd):
         w.device = device
         with pytest.raises(ValueError):
             ctx.quantize_weight_fp8(w, out)
+
+
+def test_operand_refuses_codes_of_another_format(kd):
+    """One-byte types that are not e4m3 codes are not read as such."""
+    codes, scales = torch.zeros(3, 112, dtype=torch.uint8), torch.zeros(512, dtype=torch.uint8)
+    for good in (torch.uint8, torch.float8_e4m3fn):
+        assert kd.Fp8Rows(codes.view(good), scales, 100).codes.dtype == good
+    for bad in (torch.float8_e5m2, torch.float8_e4m3fnuz, torch.int8, torch.bool):
+        with pytest.raises(ValueError):
+            kd.Fp8Rows(codes.view(bad), scales, 100)
