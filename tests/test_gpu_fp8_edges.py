@@ -104,6 +104,40 @@ def test_product_of_the_outermost_scale_bytes(ctx, kd, M):
     ctx.device_status()
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 16384, 4096), (5, 9600, 2100), (100, 16384, 1800), (256, 9600, 1700), (40, 9400, 4500)])
+def test_few_tokens_ring_used_again(ctx, kd, M, N, K):
+    """Products of few tokens whose CTAs take more blocks of 128 columns than their ring holds: stored from the sums in
+    place (1 and 5 tokens), by the join of one part (100, 256) and of two (40).  K in blocks, the CTAs to a tile, and the
+    ring's stages by shared memory are restated here, so that another plan cannot take the cases away unseen."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    blocks, tiles, nt = -(-K // 128), -(-N // 128), -(-M // 16) * 16
+    parts = min(8, blocks, max(1, sms // tiles))
+    stages = min(12, (232448 - 2048) // (128 * 128 + nt * 128 + 3 * 512))
+    assert -(-blocks // parts) > stages and parts == (2 if M == 40 else 1)
+    g = torch.Generator(device="cuda").manual_seed(K)
+    rows = []
+    for n in (M, N):
+        r = kd.Fp8Rows.empty(n, K)
+        c = torch.randint(0, 126, r.codes.shape, generator=g, device="cuda", dtype=torch.uint8)
+        c |= torch.randint(0, 2, c.shape, generator=g, device="cuda", dtype=torch.uint8) << 7
+        s = torch.randint(118, 131, (n, blocks), generator=g, device="cuda", dtype=torch.uint8)
+        r.codes.view(torch.uint8).copy_(c)
+        r.scales[torch.from_numpy(fp8_ref.tile_offsets(n, K)).cuda()] = s
+        v = torch.from_numpy(fp8_ref.VALUES).cuda()[c[:, :K].long()]
+        rows.append((r, v * torch.exp2(s.double() - 127).repeat_interleave(128, 1)[:, :K]))
+    (x, x64), (w, w64) = rows
+    bias = torch.randn(N, generator=g, device="cuda")
+    want, room = x64 @ w64.T + bias, x64.abs() @ w64.abs().T + bias.abs()
+    for name in TORCH:
+        y = torch.empty(M, N, device="cuda", dtype=TORCH[name])
+        ctx.linear_fp8(x, w, y, bias=bias)
+        lim = HALF[name] * want.abs() + (2.0 ** -25 if name == "f16" else 0) + (K + 1) * 2.0 ** -23 * room
+        big = want.abs() > 65000 if name == "f16" else torch.zeros_like(want, dtype=torch.bool)  # (beyond f16: infinite)
+        assert bool((((y.double() - want).abs() <= lim) | big).all()), name
+        assert torch.equal(y, ctx.linear_fp8(x, w, torch.empty_like(y), bias=bias))
+    ctx.device_status()
+
+
 @pytest.mark.parametrize("M", [3, 100, 300])
 def test_vectors_written_by_the_call_before(ctx, kd, M):
     """A bias that the product before wrote, and a gain likewise, in one buffer over and over: the bits that the same
