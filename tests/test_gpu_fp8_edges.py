@@ -138,6 +138,30 @@ def test_few_tokens_ring_used_again(ctx, kd, M, N, K):
     ctx.device_status()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("K,start", [(1000, 0), (1000, 1), (1537, 3), (4096, 0), (4097, 1), (5200, 0), (9000, 0), (9001, 1), (16400, 0)])
+def test_norm_in_place_over_several_warps(ctx, kd, K, start, dtype):
+    """The sum written over x and over the residual on rows of several warps, aligned and from odd starts, one and two
+    chunks a warp, more rows than CTAs: the bits of the sum and of the rows are those of a sum written elsewhere."""
+    R = 700
+    g = torch.Generator(device="cuda").manual_seed(K + start)
+    base = [torch.randn(R, start + K + 2, generator=g, device="cuda").to(TORCH[dtype]) for _ in range(2)]
+    x, res = (t[:, start:start + K] for t in base)
+    gain = 1 + 0.1 * torch.randn(K, generator=g, device="cuda")
+    h, want = torch.empty_like(x), kd.Fp8Rows.empty(R, K)
+    ctx.rms_norm_fp8(x, want, residual=res, gain=gain, h=h)
+    assert torch.equal(h, x + res)
+    for target in (0, 1):
+        wide = [t.clone() for t in base]
+        xi, ri = (t[:, start:start + K] for t in wide)
+        r = kd.Fp8Rows.empty(R, K)
+        ctx.rms_norm_fp8(xi, r, residual=ri, gain=gain, h=(xi, ri)[target])
+        assert torch.equal((xi, ri)[target], h) and torch.equal((xi, ri)[1 - target], (x, res)[1 - target])
+        for t, o in zip(wide, base):
+            assert torch.equal(t[:, :start], o[:, :start]) and torch.equal(t[:, start + K:], o[:, start + K:])
+        assert all(np.array_equal(a, b) for a, b in zip(rows_of(r), rows_of(want)))
+
+
 @pytest.mark.parametrize("M", [3, 100, 300])
 def test_vectors_written_by_the_call_before(ctx, kd, M):
     """A bias that the product before wrote, and a gain likewise, in one buffer over and over: the bits that the same
@@ -187,3 +211,61 @@ def test_written_rows_over_each_other_are_refused(ctx, kd):
         ctx.dequantize_fp8(r, v)
         assert np.array_equal(f64(v.reshape(N * L, K)), fp8_ref.decode(*rows_of(r)))
         assert int((base != 9).sum()) <= N * L * K
+
+
+def test_captured_beside_other_work(ctx, kd):
+    """Calls that may start before the one ahead of them ends, captured behind copies, fills and elementwise kernels and
+    across a fork and a join of two streams; two such graphs in turn and replayed on two streams at a time."""
+    C, F = 384, 640
+    w = operand(kd, hidden(F, C, 91) / np.sqrt(C))[0]
+    gain = dev(1 + 0.1 * seeded((C,), 92, 0))
+
+    def program(M):
+        src = torch.empty(M, C, device="cuda", dtype=torch.bfloat16)
+        x, h = torch.empty_like(src), torch.empty_like(src)
+        a, b = kd.Fp8Rows.empty(M, C), kd.Fp8Rows.empty(M, C)
+        y, z = torch.empty(M, F, device="cuda"), torch.empty(M, F, device="cuda")
+        side = torch.cuda.Stream()
+
+        def run():
+            x.copy_(src)
+            a.codes.view(torch.uint8).zero_()
+            ctx.rms_norm_fp8(x, a, gain=gain, h=h)
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                ctx.quantize_fp8(h, b)
+                ctx.linear_fp8(b, w, z)
+            ctx.linear_fp8(a, w, y)
+            torch.cuda.current_stream().wait_stream(side)
+            ctx.quantize_fp8(h, b)
+            ctx.dequantize_fp8(b, h)
+            y.add_(z)
+            x.add_(h)
+        return src, (x, h, y, z), run
+
+    graphs = []
+    for M, seed in ((40, 93), (300, 94)):
+        src, outs, run = program(M)
+        src.copy_(dev(hidden(M, C, seed), "bf16"))
+        run()  # outside a graph: what each replay has to give
+        torch.cuda.synchronize()
+        want = [t.clone() for t in outs]
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            run()
+        graphs.append((g, src, outs, want))
+    for _ in range(5):
+        for g, _, outs, _ in graphs:
+            for t in outs:
+                t.zero_()
+            g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(t, v) for _, _, outs, want in graphs for t, v in zip(outs, want))
+        streams = [torch.cuda.Stream() for _ in graphs]
+        for s, (g, _, outs, _) in zip(streams, graphs):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(t, v) for _, _, outs, want in graphs for t, v in zip(outs, want))
+    ctx.device_status()
