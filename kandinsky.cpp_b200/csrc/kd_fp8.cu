@@ -390,11 +390,17 @@ __device__ __forceinline__ P* row_at(P* base, long long m, bool even, long long 
     return reinterpret_cast<P*>(even ? b + m * nb1 : b + (m / L) * nb2 + (m % L) * nb1);
 }
 
-// Threads of the norm that an SM is to hold: 768 (80 registers) for 16-bit rows, whose loads in flight are small, 512
-// (128 registers) for f32.  31,744 x 4,096 bf16 with residual, before its arithmetic was packed (136 us since): 512
-// threads 176 us, 768 154 us, 1,024 170 us (spills).
+// Threads of the norm that an SM is to hold in CTAs of at most 256 (4,096 columns): 768 (80 registers) for 16-bit rows,
+// whose loads in flight are small, 512 (128 registers) for f32.  31,744 x 4,096 bf16 with residual, before its arithmetic
+// was packed (136 us since): 512 threads 176 us, 768 154 us, 1,024 170 us (spills).  CTAs for wider rows are bounded by
+// their own size, one to an SM: of 288 to 512 threads with 103 registers and more, above 8,192 columns of 544 to 1,024 with
+// 64, which spill.  (16,384 x 5,120 bf16 with residual 156.5 us; with two CTAs an SM in the grid, the second of which
+// waits for the first, 157.9.)
 template <typename T>
-constexpr int norm_threads() { return sizeof(T) == 2 ? 768 : 512; }
+__host__ __device__ constexpr int norm_threads() { return sizeof(T) == 2 ? 768 : 512; }
+// CTAs of `most` threads that the registers leave room for.
+template <typename T>
+__host__ __device__ constexpr int norm_ctas(int most) { return norm_threads<T>() / most > 0 ? norm_threads<T>() / most : 1; }
 
 // The sum over a warp of values >= 0 as total * 2^exponent, to 2^-26 of the largest: in whole numbers, which one
 // instruction adds exactly (in f32 the five rounded steps would be off by as much as a value's own rounding, and move
@@ -461,7 +467,7 @@ __device__ __forceinline__ void encode_again(const Norm8Params& p, long long m, 
 // in CTAs of more than 512 threads.  The CTA stays and takes every gridDim.x-th row: the gain is read once, and
 // the next row is on its way (in registers) while this one is summed, divided and written.  One pass over the data.
 template <typename T, bool kVec, int kMaxThreads, bool kWarpRows>
-__global__ void __launch_bounds__(kMaxThreads, std::max(1, norm_threads<T>() / kMaxThreads)) norm8_kernel(const __grid_constant__ Norm8Params p) {
+__global__ void __launch_bounds__(kMaxThreads, norm_ctas<T>(kMaxThreads)) norm8_kernel(const __grid_constant__ Norm8Params p) {
     constexpr int kChunks = kMaxThreads > 512 ? 2 : 1;
     constexpr bool kAhead = kChunks == 1;  // a second row of 32 columns a thread does not fit the registers
     __shared__ WarpSum part[2][32];
@@ -713,19 +719,20 @@ __global__ void __launch_bounds__(kUnitThreads) dequant8_kernel(const Dequant8Pa
 }
 
 // Up to 512 columns a warp has a row of its own; to 8,192 a CTA has a warp for every 512 columns; above, a warp for
-// every 1,024.  CTAs stay for as many rows as fill the GPU.
+// every 1,024.  As many CTAs as the GPU holds at one time, by the launch bounds, stay for all rows.
 template <typename T, bool kVec>
 cudaError_t norm8_typed(const Norm8Params& p, int num_sms, cudaStream_t st) {
     const int K = p.out.K;
     const int chunk = K <= 16 * kChunk ? kChunk : 2 * kChunk;
     const int threads = K <= kChunk ? 128 : (K + chunk - 1) / chunk * 32;
-    auto kern = K <= kChunk        ? norm8_kernel<T, kVec, 128, true>
-                : K <= 8 * kChunk  ? norm8_kernel<T, kVec, 256, false>
-                : K <= 16 * kChunk ? norm8_kernel<T, kVec, 512, false>
-                                   : norm8_kernel<T, kVec, 1024, false>;
+    const int most = K <= kChunk ? 128 : (K <= 8 * kChunk ? 256 : (K <= 16 * kChunk ? 512 : 1024));
+    auto kern = most == 128   ? norm8_kernel<T, kVec, 128, true>
+                : most == 256 ? norm8_kernel<T, kVec, 256, false>
+                : most == 512 ? norm8_kernel<T, kVec, 512, false>
+                              : norm8_kernel<T, kVec, 1024, false>;
     const long long per_cta = K <= kChunk ? 4 : 1;
     const long long want = (p.out.rows + per_cta - 1) / per_cta;
-    const long long fit = (long long)num_sms * std::max(1, norm_threads<T>() / threads);
+    const long long fit = (long long)num_sms * (most * norm_ctas<T>(most) / threads);
     return launch_following(kern, dim3((unsigned)std::min(want, fit)), (unsigned)threads, 0, 1, st, p);
 }
 
