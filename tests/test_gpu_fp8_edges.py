@@ -269,3 +269,31 @@ def test_captured_beside_other_work(ctx, kd):
         torch.cuda.synchronize()
         assert all(torch.equal(t, v) for _, _, outs, want in graphs for t, v in zip(outs, want))
     ctx.device_status()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("K,start", [(256, 0), (200, 1), (1024, 0), (1030, 1), (8448, 0)])
+def test_norm_values_beside_the_middle_of_two_codes(ctx, kd, K, start, dtype):
+    """Values within two f32 steps of the middle between two codes, on rows whose squares have an exact sum: pairs of c and
+    7 c (mean 25 c^2), so the values are g / 5 and 7 g / 5, gains placing them.  Codes are those of the exact values,
+    which f32 products with 1 / sqrt miss for some."""
+    R = 36
+    rng = np.random.default_rng(K)
+    m = np.array([1.0, 7.0])[np.arange(K) % 2]
+    middles = (17 + 2 * rng.integers(0, 8, K)) / 16.0 * 2.0 ** rng.integers(-2, 3, K)  # of normal codes: blocks reach 4 at least
+    gain = (5 * middles / m).astype(np.float32)
+    gain = (gain.view(np.int32) + rng.integers(-2, 3, K).astype(np.int32)).view(np.float32)
+    c = 1 + np.arange(R)
+    h = (c[:, None] * m[None, :]).astype(np.float32)
+    exact = np.tile(m * gain.astype(np.float64) / 5, (R, 1))
+    codes, s = fp8_ref.encode(exact)
+    inv = (1 / np.sqrt(25.0 * c.astype(np.float64) ** 2)).astype(np.float32)
+    in_f32 = fp8_ref.encode(((h * inv[:, None]) * gain[None, :]).astype(np.float64))[0]
+    assert (in_f32 != codes).sum() >= R * K // 100
+    x = torch.empty(R, start + K + 1, device="cuda", dtype=TORCH[dtype])[:, start:start + K]
+    x.copy_(dev(h))
+    r = kd.Fp8Rows.empty(R, K)
+    ctx.rms_norm_fp8(x, r, gain=dev(gain), eps=0.0)
+    got, gs = rows_of(r)
+    assert np.array_equal(gs, s)
+    assert np.array_equal(got, codes)
