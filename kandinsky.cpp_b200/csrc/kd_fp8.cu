@@ -438,7 +438,7 @@ __device__ __forceinline__ float inverse_root(float mean) {
 // The codes of some of a lane's values (bit j of `near`) once more, from h, the gain and the row's squares: |v| is above
 // the middle M between its neighbours if (h g f)^2 K > M^2 (squares + K eps), f being one over the block's scale.  The
 // comparison is in 64 bits; the squares are what the lanes' f32 chains of sixteen gave, in normal values off by 2^-25 (64
-// columns) to 2^-28 (4,096) of their sum, and never by more than 2^-20.  So codes are the exact value's where the squares
+// columns) to 2^-28 (4,096) of their sum, and never by more than 2^-19.  So codes are the exact value's where the squares
 // have an exact f32 sum, and elsewhere but for 1e-7 of all (without this 5.4e-7; elementary f32 operations 5.7e-7 to
 // 7.1e-7).  One value in 115,000 comes here.  It costs the f32 norm of 31,744 x 1,792 89 -> 100 us with its read-back and
 // the bf16 norm of 4,096 columns 196 -> 201 us: the first visits on an SM fetch instructions that the rows streaming

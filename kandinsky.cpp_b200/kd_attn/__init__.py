@@ -518,7 +518,8 @@ class Context:
 
     def rms_norm_fp8(self, x, out, residual=None, gain=None, eps=1e-6, h=None, stream=None):
         """s = x + residual (rounded to x's type, into h when given), out = s / sqrt(mean(s^2) + eps) * gain in 8
-        bits.  x, residual, h (N, L, K) of one type f32/f16/bf16; gain f32 (K,) or None; h may be x or residual."""
+        bits.  x, residual, h (N, L, K) of one type f32/f16/bf16; gain f32 (K,) or None; h may be x or residual.  Squares
+        are summed in f32: rows above about 1e19 become zeros and, with eps 0, rows below 1e-23 NaN."""
         self._here(x, residual, h, out)
         self.check(lib.kd_attn_rms_norm_fp8(self.handle, _ref(x), _ref(residual),
                                             self._vector(gain, out.in_features, "gain"), float(eps), _ref(h),

@@ -297,3 +297,25 @@ def test_norm_values_beside_the_middle_of_two_codes(ctx, kd, K, start, dtype):
     got, gs = rows_of(r)
     assert np.array_equal(gs, s)
     assert np.array_equal(got, codes)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("K", [256, 1030, 9000])
+def test_norm_rows_beyond_the_range_of_squares(ctx, kd, K, dtype):
+    """What kd_attn.h says of rows whose squares f32 does not hold; the rows beside them are as ever."""
+    x = dev(hidden(6, K, 97), dtype)
+    x[0], x[2], x[4] = 0.0, 1e-24, 1e20
+    for eps in (0.0, 1e-30):
+        r = kd.Fp8Rows.empty(6, K)
+        ctx.rms_norm_fp8(x, r, eps=eps)
+        codes, s = rows_of(r)
+        v = fp8_ref.VALUES[codes]
+        assert np.isnan(v[[0, 2]]).all() if eps == 0 else (v[0] == 0).all() and not np.isnan(v[2]).any()
+        assert (v[4] == 0).all() and (s[4] == 1).all()
+        if eps:  # 1e-24 / sqrt(1e-48 + 1e-30) = 1e-9, within half an e4m3 step and f32's last bits
+            got = fp8_ref.decode(codes[2:3], s[2:3])
+            want = float(x[2, 0].double()) / np.sqrt(float(x[2, 0].double()) ** 2 + float(np.float32(eps)))
+            assert (np.abs(got - want) <= want * (2.0 ** -4 + 2.0 ** -20)).all()
+        q = kd.Fp8Rows.empty(3, K)
+        ctx.rms_norm_fp8(x[1::2], q, eps=eps)
+        assert np.array_equal(codes[1::2], rows_of(q)[0]) and np.array_equal(s[1::2], rows_of(q)[1])
