@@ -683,7 +683,7 @@ __global__ void __launch_bounds__(kPThreads, 1)
             ++uses;
             // kWide, rows on 32-byte boundaries: a lane takes a row.  Other rows are written in pairs of columns, and
             // lanes that each wrote a row of their own would touch 32 rows with every store (30,952 x 8,194 x 1,382 bf16:
-            // 2,366 us against 412): there four lanes take eight neighbouring columns of a row.
+            // 2,366 us against 426): there four lanes take eight neighbouring columns of a row.
             constexpr int kWords = sizeof(TO) == 4 ? 32 : 16;
             uint32_t u[3 * kWords];
             if (ok) {
@@ -841,8 +841,11 @@ cudaError_t few_typed(const CUtensorMap& tmX, const CUtensorMap& tmW, const Gemm
 // Few tokens (at most 256): all of them in one tile, in steps of 16; K split over up to 8 CTAs (the portable cluster
 // size) as far as all CTAs run at one time.  (More and shorter CTAs, 3 to 7 to an SM, were slower: 16,384 x 4,096 x
 // one token 14.5 us unsplit, 19.3 us in two parts, 26 us in four.)
-// Many tokens: the tile whose rounds over the SM pairs take the fewest cycles, by the cost of a block of 128 columns
-// (MMAs for two parts of 192, copies for one of 192 or 128, as measured above) and about 1,000 cycles a tile.
+// Many tokens: the tile whose rounds over the SM pairs add up to the least, by the cost of a block of 128 columns (MMAs
+// for two parts of 192, copies for one of 192 or 128, as measured above) and 1,000 cycles a tile.  The sums rank the
+// tiles, they are not times: 1,999 tokens x 1,792 columns f16 take 29, 47 and 62 thousand cycles in one, two and three
+// rounds of 2 x 192 (850 a block, 6,000 a round and 11,000 a launch) where the sums are 12, 23 and 35, and 31,744 x 4,096 x
+// 4,096 takes 579 for 486.
 void gemm8_plan(Gemm8Params* p, int num_sms) {
     p->splits = p->parts = 1;
     p->many = p->M > kGemm8MaxTokens;
