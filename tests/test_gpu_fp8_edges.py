@@ -319,3 +319,41 @@ def test_norm_rows_beyond_the_range_of_squares(ctx, kd, K, dtype):
         q = kd.Fp8Rows.empty(3, K)
         ctx.rms_norm_fp8(x[1::2], q, eps=eps)
         assert np.array_equal(codes[1::2], rows_of(q)[0]) and np.array_equal(s[1::2], rows_of(q)[1])
+
+
+@pytest.mark.parametrize("K", [4112, 4111])
+def test_rows_past_32_bits(ctx, kd, K):
+    """Buffers of more than 2^32 elements, aligned rows and odd ones: the norm with its sum, quantising, reading back and
+    the product's output, looked at in the first and the last rows."""
+    R, tail = (1 << 20) + 77, 70
+    assert R * (K - 1) > 1 << 32
+    x = torch.zeros(R, K, device="cuda", dtype=torch.bfloat16)
+    ends = torch.cat([torch.arange(tail), torch.arange(R - tail, R)]).cuda()
+    some = dev(hidden(2 * tail, K, 98), "bf16")
+    x[ends] = some
+    r, s = kd.Fp8Rows.empty(R, K), kd.Fp8Rows.empty(2 * tail, K)
+
+    def at_ends(rows):
+        off = torch.from_numpy(fp8_ref.tile_offsets(R, K)[ends.cpu().numpy()]).cuda()
+        return rows.codes.view(torch.uint8)[ends, :K].cpu().numpy(), rows.scales[off].cpu().numpy()
+
+    ctx.quantize_fp8(x, r)
+    ctx.quantize_fp8(some, s)
+    assert all(np.array_equal(a, b) for a, b in zip(at_ends(r), rows_of(s)))
+    y = torch.full_like(x, 3.0)
+    ctx.dequantize_fp8(r, y)
+    assert torch.equal(y[ends], ctx.dequantize_fp8(s, torch.empty_like(some))) and not bool(y[tail:R - tail].any())
+    ctx.rms_norm_fp8(x, r, residual=x, h=y)
+    ctx.rms_norm_fp8(some, s, residual=some)
+    assert all(np.array_equal(a, b) for a, b in zip(at_ends(r), rows_of(s)))
+    assert torch.equal(y[ends], some + some) and not bool(y[tail:R - tail].any())
+    a, b = kd.Fp8Rows.empty(R, 128), kd.Fp8Rows.empty(2 * tail, 128)
+    few = dev(hidden(2 * tail, 128, 99))
+    wide = torch.zeros(R, 128, device="cuda")
+    wide[ends] = few
+    ctx.quantize_fp8(wide, a)
+    ctx.quantize_fp8(few, b)
+    w, _ = operand(kd, hidden(K, 128, 100))
+    ctx.linear_fp8(a, w, y)
+    assert torch.equal(y[ends], ctx.linear_fp8(b, w, torch.empty_like(some))) and not bool(y[tail:R - tail].any())
+    ctx.device_status()
